@@ -10,7 +10,8 @@ optuna_training.py:35-67).  Here one handle steps thousands of envs per call:
   stands alone with the same methods.
 * `URGymTorchVecEnv` -- device-resident rollouts: actions in, observations / rewards / flags out as torch tensors
   in HBM, every kernel ordered on the handle's HIP stream (policy forward passes included, `stream_context()`),
-  no host round trip per step.  `rollout(policy, steps)` runs a policy on the device for a batch of steps.
+  no host round trip per step.  `rollout(policy, steps)` runs a policy on the device for a batch of steps; a policy
+  with memory (`urgym_amd.policy.MemoryPolicy`) is stepped with its state and the episode starts.
 """
 import numpy as np
 
@@ -125,6 +126,7 @@ class URGymTorchVecEnv:
         self.substeps = torch.zeros(n, dtype=torch.int32, device=self.device)
         self.low = torch.as_tensor(np.asarray(self.action_space.low), dtype=torch.float32, device=self.device)
         self.high = torch.as_tensor(np.asarray(self.action_space.high), dtype=torch.float32, device=self.device)
+        self._fresh = True  # no step since the last reset: every env begins an episode
         # the buffers were zero-filled on the caller's stream; the handle's stream is non-blocking
         self.stream.wait_stream(torch.cuda.current_stream(self.device))
 
@@ -150,7 +152,12 @@ class URGymTorchVecEnv:
         cur = self._enter()
         self.sim._chk(self.sim.L.urgym_reset_device(self.sim.h, None, None, v(self.obs.data_ptr())), "urgym_reset_device")
         self._leave(cur)
+        self._fresh = True
         return self.obs
+
+    def episode_starts(self):
+        """uint8 (n,): 1 where `obs` is the first observation of an episode (after reset(), and after an autoreset)"""
+        return self.torch.ones_like(self.terminated) if self._fresh else self.terminated | self.truncated
 
     def step(self, actions):
         """actions: (n, act_dim) CUDA tensor from any stream of the env's device (the env stream waits for the
@@ -165,26 +172,50 @@ class URGymTorchVecEnv:
                              self.terminated.data_ptr(), self.truncated.data_ptr(), self.success.data_ptr(),
                              self.substeps.data_ptr())
         self._leave(cur)
+        self._fresh = False
         return self.obs, self.reward, self.terminated, self.truncated, self.final_obs
 
-    def rollout(self, policy, steps):
+    def rollout(self, policy, steps, state=None, record=False):
         """Run `policy(obs) -> actions` (a torch module / function on the device) for `steps` batched env steps
-        on the env stream; returns per-step reward sums and done counts (tensors on the device)."""
+        on the env stream; returns per-step reward sums and done counts (tensors on the device).
+
+        A policy with memory -- one that has `initial_state(envs)` and `step(obs, state, start)` -- is stepped with its
+        state (updated in place; `state`: what it remembers from the rollout before, None: nothing) and the flags of the
+        envs whose episode begins.  record=True returns a third value, what a learner needs of the rollout as time-major
+        tensors: "obs" and "action" (float32), "reward", "terminated", "truncated", "start" (uint8, the episode starts
+        that `ops.decay_attention` takes), and "state", the memory before the first step (None without memory)."""
         torch = self.torch
+        memory = hasattr(policy, "initial_state") and hasattr(policy, "step")
+        if state is not None and not memory:
+            raise TypeError("state is for a policy with memory: one that has initial_state() and step()")
         cur = self._enter()
         with self.stream_context():
             rew = torch.zeros(steps, dtype=torch.float64, device=self.device)
             done = torch.zeros(steps, dtype=torch.int64, device=self.device)
-            obs = self.obs
+            obs, rec = self.obs, None
+            if memory and state is None:
+                state = policy.initial_state(self.num_envs)
+            if record:
+                n, f32, u8 = self.num_envs, torch.float32, torch.uint8
+                rec = {name: torch.empty(steps, n, *tail, dtype=dt, device=self.device) for name, tail, dt in (
+                    ("obs", obs.shape[1:], f32), ("action", self.low.shape, f32), ("reward", (), torch.float64),
+                    ("terminated", (), u8), ("truncated", (), u8), ("start", (), u8))}
+                rec["state"] = [s.clone() for s in state] if memory else None
             for t in range(steps):
+                start = self.episode_starts() if memory or record else None
+                x = obs.to(torch.float32)
                 with torch.no_grad():
-                    act = policy(obs.to(torch.float32))
+                    act = policy.step(x, state, start) if memory else policy(x)
                 act = torch.maximum(torch.minimum(act, self.high), self.low)
                 obs, r, term, trunc, _ = self.step(act)
                 rew[t] = r.sum()
                 done[t] = (term | trunc).sum()
+                if record:
+                    for name, value in (("obs", x), ("action", act), ("reward", r), ("terminated", term), ("truncated", trunc),
+                                        ("start", start)):
+                        rec[name][t] = value
         self._leave(cur)
-        return rew, done
+        return (rew, done, rec) if record else (rew, done)
 
     def sync(self):
         self.sim.sync()
