@@ -51,8 +51,7 @@ def decay_bounds(args, kw, dtype):
     * In 32 bits: a sum of at most steps + 2 * 128 terms (u each, twice: products and sums), a power of the decay (an exponent
       of at most steps * |log_decay| rounded by u, the exponential by 2 u, once per step at the most: 4 u a step).
     * 16-bit inputs: the scores and the state inside a product are rounded to the type (u each, and one factor only in any
-      product), tokens that enter the state are held in two parts of the type (u^2, and 2^-25 absolute in fp16's subnormal
-      range, covered by the factor 2 below for the tests' values of about 1).
+      product), tokens that enter the state are held in two parts of the type (u^2).
     * The result is rounded to the type (states: float32)."""
     mags = decay_reference(*args, **kw, magnitude=True)
     refs = decay_reference(*args, **kw)

@@ -166,6 +166,30 @@ def test_an_episode_does_not_see_another(ops, dtype):
         assert ((x.double().cpu() - y.double().cpu()).abs() <= 2 * b).all()
 
 
+@pytest.mark.parametrize("dtype", ALL, ids=str)
+def test_a_step_does_not_see_a_later_one(ops, dtype):
+    """an infinity or NaN in the middle of an episode: every answer before it is as without it, and so is the gradient of every
+    step after it with respect to what does not reach it"""
+    steps, at = 75, 44
+    q, k, v, g, state, _, do, dfinal = _case(steps, 2, 2, 32, 48, dtype, 0.0, True, seed=21)
+    refs, bounds = decay_bounds((q, k, v, g, state), dict(do=do, dfinal=dfinal), dtype)
+    for x, value in ((q, float("nan")), (k, float("inf")), (v, float("nan")), (v, float("-inf"))):
+        keep = x[at].clone()
+        x[at] = value
+        got = _grads(ops, q, k, v, g, state, None, do, dfinal)
+        x[at] = keep
+        assert_close(got[0][:at], refs[0][:at], bounds[0][:at], "o")
+        assert_close(got[2][:at], refs[2][:at], bounds[2][:at], "dq")
+        assert not torch.isfinite(got[0][at].float()).all()
+    keep = do[at].clone()
+    do[at] = float("nan")  # reaches the gradients of the steps up to it only
+    got = _grads(ops, q, k, v, g, state, None, do, dfinal)
+    do[at] = keep
+    for i in (3, 4):
+        assert_close(got[i][at + 1:], refs[i][at + 1:], bounds[i][at + 1:], i)
+        assert torch.isnan(got[i][at].float()).any()
+
+
 def test_decays_at_their_ends(ops):
     """no decay at all, at once (-inf), and one so strong that its powers underflow"""
     q, k, v, _, state, start, do, dfinal = _case(50, 2, 3, 16, 16, torch.float32, 0.05, True, seed=4)
