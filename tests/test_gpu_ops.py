@@ -324,7 +324,14 @@ def test_layer_norm_strides_and_partial_gradients(ops):
     grads = torch.autograd.grad(want, (w, b), dy)
     pad = torch.zeros(6, 5, 31, device=DEV)
     pad[..., 3:27] = x
-    for v in (pad[..., 3:27], x.transpose(0, 1).contiguous().transpose(0, 1), x.transpose(0, 2).contiguous().transpose(0, 2)):
+    # rows off 16-byte alignment are summed in another order: each of the two sums is within its bound of the definition
+    refs, bounds = norm_bounds(x, w, b, 1e-5, dy)
+    off = ops.layer_norm(pad[..., 3:27], w, b)
+    for a, r, e in zip((off, *torch.autograd.grad(off, (w, b), dy)), (refs[0], *refs[2:]), (bounds[0], *bounds[2:])):
+        assert_close(a, r, e)
+    pad = torch.zeros(6, 5, 32, device=DEV)
+    pad[..., 4:28] = x
+    for v in (pad[..., 4:28], x.transpose(0, 1).contiguous().transpose(0, 1), x.transpose(0, 2).contiguous().transpose(0, 2)):
         assert torch.equal(ops.layer_norm(v, w, b), want)
         got = torch.autograd.grad(ops.layer_norm(v, w, b), (w, b), dy.transpose(0, 1).contiguous().transpose(0, 1))
         assert all(torch.equal(a, c) for a, c in zip(got, grads))

@@ -21,111 +21,400 @@ int uo_launched(const char* what) {
 
 extern "C" const char* urgym_ops_last_error(void) { return uo_message; }
 
-// One wave per row: the mean, then the centred second moment (no E[x^2] - mean^2, which cancels), then the output.
-template <typename T, typename W>
-__global__ __launch_bounds__(256) void k_norm(int64_t rows, int64_t width, const T* x, int64_t xs, const W* w, const W* b,
-                                              float eps, T* y, float* mean, float* rstd) {
-    int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / UO_WAVE;
-    int lane = threadIdx.x % UO_WAVE;
-    if (row >= rows) return;
+// A row is held by a group of G threads, K vectors of V elements each (V elements = 16 bytes, or 1 where a width, stride or
+// address is odd), so x and dy are read once from memory; the statistics are the mean, then the centred second moment of the
+// values in registers (E[x^2] - mean^2 would cancel).  Groups walk over the rows with the weights kept in registers and the next row
+// already on its way.  Both directions are bound by memory: 2 (forward) and 3 (backward) row passes.
+template <typename T, int V>
+struct Vec {
+    typedef T type __attribute__((ext_vector_type(V)));
+};
+template <typename T>
+struct Vec<T, 1> {
+    typedef T type;
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void norm_load(float* to, const T* p) {
+    typename Vec<T, V>::type v = *(const typename Vec<T, V>::type*)p;
+    if constexpr (V == 1) to[0] = (float)v;
+    else
+#pragma unroll
+        for (int e = 0; e < V; e++) to[e] = (float)v[e];
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void norm_store(T* p, const float* from) {
+    typename Vec<T, V>::type v;
+    if constexpr (V == 1) v = (T)from[0];
+    else
+#pragma unroll
+        for (int e = 0; e < V; e++) v[e] = (T)from[e];
+    *(typename Vec<T, V>::type*)p = v;
+}
+
+// element i of a parameter vector of dtype wdtype, or `none` without one
+__device__ __forceinline__ float norm_param(const void* w, int wdtype, int64_t i, float none) {
+    return !w ? none : wdtype == URGYM_OPS_F32 ? ((const float*)w)[i] : wdtype == URGYM_OPS_BF16 ? (float)((const bf16*)w)[i] : (float)((const f16*)w)[i];
+}
+
+// elements i .. i + V - 1 of a parameter vector (16-byte aligned where V > 1)
+template <typename T, int V>
+__device__ __forceinline__ void norm_params(float* to, const void* w, int wdtype, int64_t i, float none) {
+    if (!w) {
+#pragma unroll
+        for (int e = 0; e < V; e++) to[e] = none;
+    } else if (wdtype == URGYM_OPS_F32) {
+        constexpr int N = V < 4 ? V : 4;
+#pragma unroll
+        for (int e = 0; e < V; e += N) norm_load<float, N>(to + e, (const float*)w + i + e);
+    } else {
+        norm_load<T, V>(to, (const T*)w + i);
+    }
+}
+
+// the sum over the G threads of a group, the same in all of them; G > 64: over the workgroup, through lds (two slots for each wave,
+// used in turn, so one barrier a sum is enough)
+template <int G>
+__device__ __forceinline__ float group_sum(float x, float* lds) {
+    x = uo_group_sum<G < UO_WAVE ? G : UO_WAVE>(x);
+    if constexpr (G > UO_WAVE) {
+        if (threadIdx.x % UO_WAVE == 0) lds[threadIdx.x / UO_WAVE] = x;
+        __syncthreads();
+        x = 0.f;
+#pragma unroll
+        for (int i = 0; i < G / UO_WAVE; i++) x += lds[i];
+    }
+    return x;
+}
+
+template <typename T, int G, int K, int V>
+__global__ __launch_bounds__(G > 256 ? G : 256) void k_norm(int64_t rows, int64_t width, const T* x, int64_t xs, const void* w,
+                                                            const void* b, int wdtype, float eps, T* y, float* mean, float* rstd) {
+    constexpr int BLOCK = G > 256 ? G : 256;
+    __shared__ float lds[2][G > UO_WAVE ? G / UO_WAVE : 1];
+    int t = threadIdx.x % G;
+    int64_t row = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G, stride = (int64_t)gridDim.x * (BLOCK / G);
+    float wv[K][V], bv[K][V], next[K][V];
+    const float inv = 1.f / (float)width;
+    bool have[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        int64_t i = (int64_t)(k * G + t) * V;
+        have[k] = i < width;
+#pragma unroll
+        for (int e = 0; e < V; e++) wv[k][e] = bv[k][e] = next[k][e] = 0.f;
+        if (have[k]) {
+            if (row < rows) norm_load<T, V>(next[k], x + row * xs + i);
+            norm_params<T, V>(wv[k], w, wdtype, i, 1.f);
+            norm_params<T, V>(bv[k], b, wdtype, i, 0.f);
+        }
+    }
+    for (; row < rows; row += stride) {
+        float v[K][V], s = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+#pragma unroll
+            for (int e = 0; e < V; e++) v[k][e] = next[k][e], s += v[k][e];
+            if (have[k] && row + stride < rows) norm_load<T, V>(next[k], x + (row + stride) * xs + (int64_t)(k * G + t) * V);
+        }
+        float mu = group_sum<G>(s, lds[0]) / (float)width, q = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; k++)
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                v[k][e] -= mu;
+                if (have[k]) q += v[k][e] * v[k][e];
+            }
+        float r = rsqrtf(group_sum<G>(q, lds[1]) * inv + eps);
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+#pragma unroll
+            for (int e = 0; e < V; e++) v[k][e] = v[k][e] * r * wv[k][e] + bv[k][e];
+            if (have[k]) norm_store<T, V>(y + row * width + (int64_t)(k * G + t) * V, v[k]);
+        }
+        if (mean && t == 0) mean[row] = mu, rstd[row] = r;
+    }
+}
+
+// dx, and in the same pass the workgroup's sums of dy xh and dy over its rows, in registers, to ws[0 / 1][workgroup][width]; the
+// sums over workgroups are k_norm_dw_sum's.
+template <typename T, int G, int K, int V>
+__global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_back(int64_t rows, int64_t width, const T* dy, int64_t ds, const T* x,
+                                                                 int64_t xs, const void* w, int wdtype, const float* mean,
+                                                                 const float* rstd, T* dx, float* ws) {
+    constexpr int BLOCK = G > 256 ? G : 256;
+    __shared__ float lds[2][G > UO_WAVE ? G / UO_WAVE : 1];
+    __shared__ float cols[G > UO_WAVE ? 1 : 2 * 4 * G * K * V];
+    int t = threadIdx.x % G;
+    int64_t row = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G, stride = (int64_t)gridDim.x * (BLOCK / G);
+    float wv[K][V], dw[K][V], db[K][V], nx[K][V], nd[K][V], n_mu = 0.f, n_r = 0.f;
+    const float inv = 1.f / (float)width;
+    bool have[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        int64_t i = (int64_t)(k * G + t) * V;
+        have[k] = i < width;
+#pragma unroll
+        for (int e = 0; e < V; e++) wv[k][e] = dw[k][e] = db[k][e] = nx[k][e] = nd[k][e] = 0.f;
+        if (have[k]) {
+            if (row < rows) norm_load<T, V>(nx[k], x + row * xs + i), norm_load<T, V>(nd[k], dy + row * ds + i);
+            norm_params<T, V>(wv[k], w, wdtype, i, 1.f);
+        }
+    }
+    if (row < rows) n_mu = mean[row], n_r = rstd[row];
+    for (; row < rows; row += stride) {
+        float h[K][V], d[K][V], mu = n_mu, r = n_r, sg = 0.f, sh = 0.f;
+        bool more = row + stride < rows;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                h[k][e] = (nx[k][e] - mu) * r, d[k][e] = nd[k][e];
+                if (have[k]) {
+                    dw[k][e] += d[k][e] * h[k][e], db[k][e] += d[k][e];
+                    float gr = d[k][e] * wv[k][e];
+                    sg += gr, sh += gr * h[k][e];
+                }
+            }
+            int64_t i = (int64_t)(k * G + t) * V;
+            if (have[k] && more) norm_load<T, V>(nx[k], x + (row + stride) * xs + i), norm_load<T, V>(nd[k], dy + (row + stride) * ds + i);
+        }
+        if (more) n_mu = mean[row + stride], n_r = rstd[row + stride];
+        if (!dx) continue;
+        sg = group_sum<G>(sg, lds[0]) * inv;
+        sh = group_sum<G>(sh, lds[1]) * inv;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+#pragma unroll
+            for (int e = 0; e < V; e++) h[k][e] = r * (d[k][e] * wv[k][e] - sg - h[k][e] * sh);
+            if (have[k]) norm_store<T, V>(dx + row * width + (int64_t)(k * G + t) * V, h[k]);
+        }
+    }
+    if (!ws) return;
+    float* out = ws + (int64_t)blockIdx.x * width;
+    int64_t half = (int64_t)gridDim.x * width;
+    if constexpr (G > UO_WAVE) {
+#pragma unroll
+        for (int k = 0; k < K; k++)
+            if (have[k])
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    int64_t i = (int64_t)(k * G + t) * V + e;
+                    out[i] = dw[k][e], out[half + i] = db[k][e];
+                }
+    } else {  // the wave's groups first, then the four waves
+        int wave = threadIdx.x / UO_WAVE;
+#pragma unroll
+        for (int k = 0; k < K; k++)
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                float p = dw[k][e], q = db[k][e];
+#pragma unroll
+                for (int m = G; m < UO_WAVE; m *= 2) p += __shfl_xor(p, m), q += __shfl_xor(q, m);
+                if (threadIdx.x % UO_WAVE < G) {
+                    int i = (k * G + t) * V + e;
+                    cols[wave * G * K * V + i] = p, cols[(4 + wave) * G * K * V + i] = q;
+                }
+            }
+        __syncthreads();
+        for (int i = threadIdx.x; i < width; i += BLOCK) {
+            float p = 0.f, q = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) p += cols[j * G * K * V + i], q += cols[(4 + j) * G * K * V + i];
+            out[i] = p, out[half + i] = q;
+        }
+    }
+}
+
+// Rows that no group holds (more than 4096 vectors, or 8192 odd elements): one workgroup a row, the row read again for each pass.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_norm_wide(int64_t width, const T* x, int64_t xs, const void* w, const void* b, int wdtype,
+                                                    float eps, T* y, float* mean, float* rstd) {
+    __shared__ float lds[2][16];
+    int64_t row = blockIdx.x;
     const T* xr = x + row * xs;
-    float s = 0.f;
-    for (int64_t i = lane; i < width; i += UO_WAVE) s += (float)xr[i];
-    float mu = uo_wave_sum(s) / (float)width;
-    float q = 0.f;
-    for (int64_t i = lane; i < width; i += UO_WAVE) {
-        float c = (float)xr[i] - mu;
-        q += c * c;
-    }
-    float r = 1.0f / sqrtf(uo_wave_sum(q) / (float)width + eps);
-    for (int64_t i = lane; i < width; i += UO_WAVE)
-        y[row * width + i] = (T)(((float)xr[i] - mu) * r * (w ? (float)w[i] : 1.f) + (b ? (float)b[i] : 0.f));
-    if (mean && lane == 0) mean[row] = mu, rstd[row] = r;
+    float s = 0.f, q = 0.f;
+    for (int64_t i = threadIdx.x; i < width; i += 1024) s += (float)xr[i];
+    float mu = group_sum<1024>(s, lds[0]) / (float)width;
+    for (int64_t i = threadIdx.x; i < width; i += 1024) q += ((float)xr[i] - mu) * ((float)xr[i] - mu);
+    float r = 1.0f / sqrtf(group_sum<1024>(q, lds[1]) / (float)width + eps);
+    for (int64_t i = threadIdx.x; i < width; i += 1024)
+        y[row * width + i] = (T)(((float)xr[i] - mu) * r * norm_param(w, wdtype, i, 1.f) + norm_param(b, wdtype, i, 0.f));
+    if (mean && threadIdx.x == 0) mean[row] = mu, rstd[row] = r;
 }
-
-template <typename T, typename W>
-__global__ __launch_bounds__(256) void k_norm_dx(int64_t rows, int64_t width, const T* dy, int64_t ds, const T* x, int64_t xs,
-                                                 const W* w, const float* mean, const float* rstd, T* dx) {
-    int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / UO_WAVE;
-    int lane = threadIdx.x % UO_WAVE;
-    if (row >= rows) return;
-    const T *xr = x + row * xs, *dr = dy + row * ds;
-    float mu = mean[row], r = rstd[row], sg = 0.f, sh = 0.f;
-    for (int64_t i = lane; i < width; i += UO_WAVE) {
-        float g = (float)dr[i] * (w ? (float)w[i] : 1.f);
-        sg += g;
-        sh += g * (((float)xr[i] - mu) * r);
-    }
-    sg = uo_wave_sum(sg) / (float)width;
-    sh = uo_wave_sum(sh) / (float)width;
-    for (int64_t i = lane; i < width; i += UO_WAVE) {
-        float g = (float)dr[i] * (w ? (float)w[i] : 1.f);
-        dx[row * width + i] = (T)(r * (g - sg - ((float)xr[i] - mu) * r * sh));
-    }
-}
-
-// The rows are cut into `parts` equal runs; part p's column sums go to ws[p], then k_norm_dw_sum adds the parts in order.
-static int64_t norm_parts(int64_t rows) { return rows < 16 * 256 ? (rows + 15) / 16 : 256; }
 
 template <typename T>
-__global__ __launch_bounds__(64) void k_norm_dw(int64_t rows, int64_t width, const T* dy, int64_t ds, const T* x, int64_t xs,
-                                                const float* mean, const float* rstd, float* ws) {
+__global__ __launch_bounds__(1024) void k_norm_wide_dx(int64_t width, const T* dy, int64_t ds, const T* x, int64_t xs, const void* w,
+                                                       int wdtype, const float* mean, const float* rstd, T* dx) {
+    __shared__ float lds[2][16];
+    int64_t row = blockIdx.x;
+    const T *xr = x + row * xs, *dr = dy + row * ds;
+    float mu = mean[row], r = rstd[row], sg = 0.f, sh = 0.f;
+    for (int64_t i = threadIdx.x; i < width; i += 1024) {
+        float g = (float)dr[i] * norm_param(w, wdtype, i, 1.f);
+        sg += g, sh += g * (((float)xr[i] - mu) * r);
+    }
+    sg = group_sum<1024>(sg, lds[0]) / (float)width;
+    sh = group_sum<1024>(sh, lds[1]) / (float)width;
+    for (int64_t i = threadIdx.x; i < width; i += 1024)
+        dx[row * width + i] = (T)(r * ((float)dr[i] * norm_param(w, wdtype, i, 1.f) - sg - ((float)xr[i] - mu) * r * sh));
+}
+
+template <typename T>
+__global__ __launch_bounds__(64) void k_norm_wide_dw(int64_t rows, int64_t width, const T* dy, int64_t ds, const T* x, int64_t xs,
+                                                     const float* mean, const float* rstd, float* ws) {
     int64_t c = (int64_t)blockIdx.y * 64 + threadIdx.x, parts = gridDim.x, p = blockIdx.x;
     if (c >= width) return;
     float dw = 0.f, db = 0.f;
     for (int64_t r = rows * p / parts; r < rows * (p + 1) / parts; r++) {
         float d = (float)dy[r * ds + c];
-        dw += d * (((float)x[r * xs + c] - mean[r]) * rstd[r]);
-        db += d;
+        dw += d * (((float)x[r * xs + c] - mean[r]) * rstd[r]), db += d;
     }
     ws[p * width + c] = dw;
     ws[(parts + p) * width + c] = db;
 }
 
-template <typename W>
-__global__ __launch_bounds__(64) void k_norm_dw_sum(int64_t width, int64_t parts, const float* ws, W* dw, W* db) {
-    int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x;
-    if (c >= width) return;
-    float a = 0.f, b = 0.f;
-    for (int64_t p = 0; p < parts; p++) a += ws[p * width + c], b += ws[(parts + p) * width + c];
-    if (dw) dw[c] = (W)a;
-    if (db) db[c] = (W)b;
+// the workgroups' sums added up in a fixed order: 32 columns by 32 runs of parts to a workgroup, the runs then through LDS
+__global__ __launch_bounds__(1024) void k_norm_dw_sum(int64_t width, int64_t parts, const float* ws, void* dw, void* db, int wdtype) {
+    __shared__ float lds[32][33];
+    void* to = blockIdx.y ? db : dw;
+    if (!to) return;
+    int c = threadIdx.x % 32, run = threadIdx.x / 32;
+    int64_t col = (int64_t)blockIdx.x * 32 + c;
+    const float* p = ws + blockIdx.y * parts * width + col;
+    float s = 0.f;
+    if (col < width)
+#pragma unroll 8
+        for (int64_t i = run; i < parts; i += 32) s += p[i * width];
+    lds[run][c] = s;
+    __syncthreads();
+    s = uo_group_sum<32>(lds[c][run]);  // thread (run, c) sums column `run` over its 32 runs
+    col = (int64_t)blockIdx.x * 32 + run;
+    if (c || col >= width) return;
+    if (wdtype == URGYM_OPS_F32) ((float*)to)[col] = s;
+    else if (wdtype == URGYM_OPS_BF16) ((bf16*)to)[col] = (bf16)s;
+    else ((f16*)to)[col] = (f16)s;
 }
 
 static int norm_check(const char* what, int dtype, int wdtype, int64_t rows, int64_t width) {
     if (dtype < 0 || dtype > 2 || wdtype < 0 || wdtype > 2) return uo_fail("%s: unknown dtype %d / %d", what, dtype, wdtype);
     if (wdtype != dtype && wdtype != URGYM_OPS_F32) return uo_fail("%s: the weight's dtype is x's or float32", what);
     if (rows < 0 || width < 1) return uo_fail("%s: rows %lld, width %lld", what, (long long)rows, (long long)width);
-    if (width > (1 << 20) || rows > ((int64_t)1 << 32)) return uo_fail("%s: rows %lld x width %lld is too large", what, (long long)rows, (long long)width);
+    if (width > (1 << 20) || rows > ((int64_t)1 << 30)) return uo_fail("%s: rows %lld x width %lld is too large", what, (long long)rows, (long long)width);
     return 0;
 }
 
-template <typename T, typename W>
-static int norm_fwd(int64_t rows, int64_t width, const void* x, int64_t xs, const void* w, const void* b, float eps, void* y,
+// The group that holds a row of `units` vectors: one vector a thread up to a wave, then more; workgroups of 256 and 1024 threads for
+// wide rows.  Single elements (odd widths) are small work a thread, so a thread takes 4 or 8 of them before the group grows.
+template <bool VECTOR, typename F>
+static bool norm_group(int64_t units, F&& f) {
+#define TRY(most, G, K) \
+    if (units <= most) { \
+        f.template operator()<G, K>(); \
+        return true; \
+    }
+    if constexpr (VECTOR) {
+        TRY(8, 8, 1) TRY(16, 16, 1) TRY(32, 32, 1) TRY(64, 64, 1) TRY(128, 64, 2) TRY(256, 256, 1) TRY(512, 256, 2) TRY(768, 256, 3)
+        TRY(1024, 256, 4) TRY(2048, 1024, 2) TRY(4096, 1024, 4)
+    } else {
+        TRY(8, 8, 1) TRY(16, 8, 2) TRY(32, 8, 4) TRY(64, 16, 4) TRY(128, 32, 4) TRY(256, 64, 4) TRY(512, 64, 8) TRY(1024, 256, 4)
+        TRY(2048, 256, 8) TRY(4096, 1024, 4) TRY(8192, 1024, 8)
+    }
+#undef TRY
+    return false;
+}
+
+// workgroups of the forward pass: enough to fill the chip, several rows each beyond that
+static unsigned norm_blocks(int64_t rows, int per_block, int block) {
+    int64_t n = (rows + per_block - 1) / per_block, most = 256 * 2048 / block;
+    return (unsigned)(n < most ? n : most);
+}
+
+// Workgroups of the backward pass, each of which leaves a part of the column sums: half of what fills the chip, so that parts (two
+// floats a column) stay small beside the rows.
+static int64_t norm_parts(int64_t rows, int64_t width) {
+    int64_t rows_a_time = width <= 512 ? 8 : 1, most = width <= 512 ? 1024 : 512, n = (rows + rows_a_time - 1) / rows_a_time;
+    return n < most ? n : most;
+}
+
+template <typename T, int V>
+struct NormForward {
+    int64_t rows, width;
+    const void* x;
+    int64_t xs;
+    const void *w, *b;
+    int wdtype;
+    float eps;
+    void* y;
+    float *mean, *rstd;
+    hipStream_t st;
+    template <int G, int K>
+    void operator()() {
+        constexpr int block = G > 256 ? G : 256;
+        k_norm<T, G, K, V><<<norm_blocks(rows, block / G, block), block, 0, st>>>(rows, width, (const T*)x, xs, w, b, wdtype, eps, (T*)y, mean, rstd);
+    }
+};
+
+template <typename T, int V>
+struct NormBackward {
+    int64_t rows, width;
+    const void* dy;
+    int64_t ds;
+    const void* x;
+    int64_t xs;
+    const void* w;
+    int wdtype;
+    const float *mean, *rstd;
+    void* dx;
+    float* ws;
+    hipStream_t st;
+    template <int G, int K>
+    void operator()() {
+        constexpr int block = G > 256 ? G : 256;
+        k_norm_back<T, G, K, V><<<(unsigned)norm_parts(rows, width), block, 0, st>>>(rows, width, (const T*)dy, ds, (const T*)x, xs, w, wdtype, mean, rstd, (T*)dx, ws);
+    }
+};
+
+// whether rows (or, with stride 0, a parameter vector) can be read and written as 16-byte vectors of `n` elements
+static bool norm_vectors(int64_t width, int64_t stride, const void* p, int n) { return width % n == 0 && stride % n == 0 && (uintptr_t)p % 16 == 0; }
+
+template <typename T>
+static int norm_fwd(int64_t rows, int64_t width, const void* x, int64_t xs, const void* w, const void* b, int wdtype, float eps, void* y,
                     float* mean, float* rstd, hipStream_t st) {
-    k_norm<T, W><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(rows, width, (const T*)x, xs, (const W*)w, (const W*)b, eps, (T*)y, mean, rstd);
+    constexpr int V = 16 / sizeof(T);
+    bool done;
+    if (norm_vectors(width, xs, x, V) && norm_vectors(width, width, y, V) && norm_vectors(width, 0, w, V) && norm_vectors(width, 0, b, V))
+        done = norm_group<true>(width / V, NormForward<T, V>{rows, width, x, xs, w, b, wdtype, eps, y, mean, rstd, st});
+    else
+        done = norm_group<false>(width, NormForward<T, 1>{rows, width, x, xs, w, b, wdtype, eps, y, mean, rstd, st});
+    if (!done) k_norm_wide<T><<<(unsigned)rows, 1024, 0, st>>>(width, (const T*)x, xs, w, b, wdtype, eps, (T*)y, mean, rstd);
     return uo_launched("urgym_ops_layer_norm");
 }
 
-template <typename T, typename W>
-static int norm_bwd(int64_t rows, int64_t width, const void* dy, int64_t ds, const void* x, int64_t xs, const void* w,
+template <typename T>
+static int norm_bwd(int64_t rows, int64_t width, const void* dy, int64_t ds, const void* x, int64_t xs, const void* w, int wdtype,
                     const float* mean, const float* rstd, void* dx, void* dw, void* db, float* ws, hipStream_t st) {
-    if (dx && rows)
-        k_norm_dx<T, W><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(rows, width, (const T*)dy, ds, (const T*)x, xs, (const W*)w, mean, rstd, (T*)dx);
-    if (dw || db) {
-        int64_t parts = norm_parts(rows);
-        unsigned cols = (unsigned)((width + 63) / 64);
-        if (parts) k_norm_dw<T><<<dim3((unsigned)parts, cols), 64, 0, st>>>(rows, width, (const T*)dy, ds, (const T*)x, xs, mean, rstd, ws);
-        k_norm_dw_sum<W><<<cols, 64, 0, st>>>(width, parts, ws, (W*)dw, (W*)db);
+    constexpr int V = 16 / sizeof(T);
+    int64_t parts = norm_parts(rows, width);
+    if (!dw && !db) ws = nullptr;
+    if (rows && (dx || ws)) {
+        bool done;
+        if (norm_vectors(width, xs, x, V) && norm_vectors(width, ds, dy, V) && norm_vectors(width, width, dx, V) && norm_vectors(width, 0, w, V))
+            done = norm_group<true>(width / V, NormBackward<T, V>{rows, width, dy, ds, x, xs, w, wdtype, mean, rstd, dx, ws, st});
+        else
+            done = norm_group<false>(width, NormBackward<T, 1>{rows, width, dy, ds, x, xs, w, wdtype, mean, rstd, dx, ws, st});
+        if (!done && dx) k_norm_wide_dx<T><<<(unsigned)rows, 1024, 0, st>>>(width, (const T*)dy, ds, (const T*)x, xs, w, wdtype, mean, rstd, (T*)dx);
+        if (!done && ws)
+            k_norm_wide_dw<T><<<dim3((unsigned)parts, (unsigned)((width + 63) / 64)), 64, 0, st>>>(rows, width, (const T*)dy, ds, (const T*)x, xs, mean, rstd, ws);
     }
+    if (dw || db) k_norm_dw_sum<<<dim3((unsigned)((width + 31) / 32), 2), 1024, 0, st>>>(width, parts, ws, dw, db, wdtype);
     return uo_launched("urgym_ops_layer_norm_backward");
 }
 
-// calls F<T, W>(args...) for the dtype pair (wdtype is dtype or float32)
-#define NORM_DISPATCH(F, ...)                                                      \
-    (dtype == URGYM_OPS_F32    ? F<float, float>(__VA_ARGS__)                      \
-     : dtype == URGYM_OPS_BF16 ? (wdtype ? F<bf16, bf16>(__VA_ARGS__) : F<bf16, float>(__VA_ARGS__)) \
-                               : (wdtype ? F<f16, f16>(__VA_ARGS__) : F<f16, float>(__VA_ARGS__)))
+// calls F<T>(args...) for x's dtype
+#define NORM_DISPATCH(F, ...) \
+    (dtype == URGYM_OPS_F32 ? F<float>(__VA_ARGS__) : dtype == URGYM_OPS_BF16 ? F<bf16>(__VA_ARGS__) : F<f16>(__VA_ARGS__))
 
 extern "C" int urgym_ops_layer_norm(int dtype, int wdtype, int64_t rows, int64_t width, const void* x, int64_t x_stride,
                                     const void* weight, const void* bias, float eps, void* y, float* mean, float* rstd,
@@ -133,10 +422,10 @@ extern "C" int urgym_ops_layer_norm(int dtype, int wdtype, int64_t rows, int64_t
     if (norm_check("urgym_ops_layer_norm", dtype, wdtype, rows, width)) return -1;
     if (!rows) return 0;
     if (!x || !y || !mean != !rstd) return uo_fail("urgym_ops_layer_norm: x and y are needed, mean and rstd go together");
-    return NORM_DISPATCH(norm_fwd, rows, width, x, x_stride, weight, bias, eps, y, mean, rstd, (hipStream_t)stream);
+    return NORM_DISPATCH(norm_fwd, rows, width, x, x_stride, weight, bias, wdtype, eps, y, mean, rstd, (hipStream_t)stream);
 }
 
-extern "C" int64_t urgym_ops_layer_norm_workspace(int64_t rows, int64_t width) { return rows < 0 || width < 1 ? 0 : 2 * norm_parts(rows) * width; }
+extern "C" int64_t urgym_ops_layer_norm_workspace(int64_t rows, int64_t width) { return rows < 0 || width < 1 ? 0 : 2 * norm_parts(rows, width) * width; }
 
 extern "C" int urgym_ops_layer_norm_backward(int dtype, int wdtype, int64_t rows, int64_t width, const void* dy, int64_t dy_stride,
                                              const void* x, int64_t x_stride, const void* weight, const float* mean,
@@ -145,6 +434,6 @@ extern "C" int urgym_ops_layer_norm_backward(int dtype, int wdtype, int64_t rows
     if (norm_check("urgym_ops_layer_norm_backward", dtype, wdtype, rows, width)) return -1;
     if (rows && (!dy || !x || !mean || !rstd)) return uo_fail("urgym_ops_layer_norm_backward: dy, x, mean and rstd are needed");
     if (rows && (dweight || dbias) && !workspace) return uo_fail("urgym_ops_layer_norm_backward: a workspace is needed");
-    return NORM_DISPATCH(norm_bwd, rows, width, dy, dy_stride, x, x_stride, weight, mean, rstd, dx, dweight, dbias, workspace,
-                         (hipStream_t)stream);
+    return NORM_DISPATCH(norm_bwd, rows, width, dy, dy_stride, x, x_stride, weight, wdtype, mean, rstd, dx, dweight, dbias,
+                         workspace, (hipStream_t)stream);
 }
