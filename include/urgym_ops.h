@@ -55,7 +55,7 @@ typedef struct {
     float scale;
 } urgym_ops_seq;
 
-/* float32 elements of workspace for urgym_ops_decay / urgym_ops_decay_backward (0: none needed, NULL may be passed). */
+/* float32 elements of workspace for urgym_ops_decay / urgym_ops_decay_backward (0: none needed, NULL may be passed; <0: error). */
 int64_t urgym_ops_decay_workspace(const urgym_ops_seq* s, int backward);
 
 /* S_t = exp(log_decay) S_{t-1} + k_t v_t^T (S_{t-1} = 0 where start_t), o_t = scale S_t^T q_t.

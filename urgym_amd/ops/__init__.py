@@ -238,6 +238,8 @@ def _seq(q, k, v, log_decay, state, start, scale):
 
 def _workspace(s, backward, device):
     n = lib().urgym_ops_decay_workspace(ctypes.byref(s), backward)
+    if n < 0:
+        _check(-1)
     return torch.empty(n, dtype=torch.float32, device=device) if n else None
 
 

@@ -48,10 +48,14 @@ struct Sweep {
 
 struct Sweeps {
     Sweep w[3];
-    int count, slices;  // sweeps in this launch, waves for each of them
-    int heads;
-    int64_t steps, items;  // items: envs * heads * count * slices waves
+    unsigned count, slices, segs, heads;  // sweeps in this launch, waves for each of them and segment of the axis, segments
+    unsigned items;                       // envs * heads * count * slices * segs waves
+    int seg_len;                          // steps in a segment (the last may be shorter)
+    int64_t steps;
     const float* log_decay;
+    // segs > 1: for each wave what its segment adds to the state, or (after k_join) the state it begins with, as the wave's
+    // accumulators lie in its registers; and the factor that it leaves of the state before it
+    float *ws, *left;
 };
 
 template <typename T>
@@ -105,6 +109,24 @@ __device__ __forceinline__ void fetch(T* to, const T* p, int col, int width) {
     }
 }
 
+// N elements, or zeros where the mask is zero (a selection: nothing of what is dropped is computed with)
+template <typename T, int N>
+__device__ __forceinline__ void only(T* x, unsigned mask) {
+    constexpr int U = 4 / sizeof(T);
+    typedef T V __attribute__((ext_vector_type(U)));
+#pragma unroll
+    for (int i = 0; i < N; i += U) {
+        if constexpr (U == 1) {
+            x[i] = __uint_as_float(__float_as_uint(x[i]) & mask);
+        } else {
+            V v;
+            v[0] = x[i], v[1] = x[i + 1];
+            v = __builtin_bit_cast(V, __builtin_bit_cast(unsigned, v) & mask);
+            x[i] = v[0], x[i + 1] = v[1];
+        }
+    }
+}
+
 __device__ __forceinline__ float wave_max(float x) {
 #pragma unroll
     for (int m = 32; m; m >>= 1) x = fmaxf(x, __shfl_xor(x, m));
@@ -120,41 +142,59 @@ __device__ __forceinline__ void unit(float most, float* down, float* up) {
     *down = __uint_as_float(0x7f000000u - e);
 }
 
-template <typename T, int DA, int MODE>
+// element (i, j) of the state that enters the sweep
+__device__ __forceinline__ float entering(const Sweep& w, unsigned nh, int i, int j) {
+    return w.s_in && i < w.da && j < w.db ? w.in_mul * w.s_in[(int64_t)nh * w.da * w.db + i * w.s_i + j * w.s_j] : 0.f;
+}
+
+// element (r, u, v) of a wave's accumulators in ws: float4s, lane by lane
+__device__ __forceinline__ f4* held(const Sweeps& all, unsigned item, int tiles, int tile, int lane) {
+    return (f4*)all.ws + ((int64_t)item * tiles + tile) * UO_WAVE + lane;
+}
+
+// STATE: only what the segment adds to the state (no a, no o); segments after it need that before they can begin.
+template <typename T, int DA, int MODE, bool STATE>
 __global__ __launch_bounds__(256) void k_sweep(Sweeps all) {
     typedef typename Kind<T>::Frag Frag;
     constexpr int FE = Kind<T>::FE, NB = FE / 4, CH = 16 * NB, NF = DA / 4 / FE, VA = DA / 16, VB = 2;
     constexpr bool HALF = sizeof(T) == 2, F16 = HALF && T(1.0 / 1024 + 1) != T(1);
-    int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / UO_WAVE);
+    unsigned item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / UO_WAVE);
     if (item >= all.items) return;
-    int slice = item % all.slices, role = item / all.slices % all.count;
-    int64_t nh = item / (all.slices * all.count), n = nh / all.heads;
-    int h = nh % all.heads, lane = threadIdx.x % UO_WAVE, c = lane % 16, g = lane / 16;
+    // neighbours share their rows: the slices, then the sweeps, then the heads of one env
+    unsigned slice = item % all.slices, rest = item / all.slices, role = rest % all.count, nhs = rest / all.count;
+    unsigned nh = nhs / all.segs, seg = nhs % all.segs, h = nh % all.heads;
+    int64_t n = nh / all.heads;
+    int lane = threadIdx.x % UO_WAVE, c = lane % 16, g = lane / 16;
     const Sweep& w = all.w[role];
     int j0 = slice * 16 * VB;
     if (j0 >= w.db) return;
     const int col = j0 + VB * c, da = w.da, db = w.db;
-    const int64_t steps = all.steps;
+    const int64_t x0 = (int64_t)seg * all.seg_len, left_steps = all.steps - x0;
+    const int steps = left_steps < all.seg_len ? (int)left_steps : all.seg_len;
     float lg = all.log_decay[h] * 1.44269504088896340736f;
 
     // lane pointers: a row's part (token c), and neighbouring columns of token 4 g
-    const T* pa = (const T*)w.a.p + n * w.a.sn + h * w.a.sh + c * w.a.st + g * (DA / 4);
-    const T* pb = (const T*)w.b.p + n * w.b.sn + h * w.b.sh + c * w.b.st + g * (DA / 4);
-    const T* pbt = (const T*)w.b.p + n * w.b.sn + h * w.b.sh + 4 * g * w.b.st + VA * c;
-    const T* pct = (const T*)w.c.p + n * w.c.sn + h * w.c.sh + 4 * g * w.c.st + col;
-    T* po = (T*)w.o.p + n * w.o.sn + h * w.o.sh + 4 * g * w.o.st + col;
+    const T* pa = (const T*)w.a.p + n * w.a.sn + h * w.a.sh + (x0 + c) * w.a.st + g * (DA / 4);
+    const T* pb = (const T*)w.b.p + n * w.b.sn + h * w.b.sh + (x0 + c) * w.b.st + g * (DA / 4);
+    const T* pbt = (const T*)w.b.p + n * w.b.sn + h * w.b.sh + (x0 + 4 * g) * w.b.st + VA * c;
+    const T* pct = (const T*)w.c.p + n * w.c.sn + h * w.c.sh + (x0 + 4 * g) * w.c.st + col;
+    T* po = (T*)w.o.p + n * w.o.sn + h * w.o.sh + (x0 + 4 * g) * w.o.st + col;
     const int64_t sta = w.a.st, stb = w.b.st, stc = w.c.st, sto = w.o.st;
 
     f4 S[VA][VB];
 #pragma unroll
     for (int u = 0; u < VA; u++)
 #pragma unroll
-        for (int v = 0; v < VB; v++)
+        for (int v = 0; v < VB; v++) {
+            if (STATE) {
+                S[u][v] = (f4)0.f;
+            } else if (all.segs > 1) {
+                S[u][v] = *held(all, item, VA * VB, u * VB + v, lane);
+            } else {
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                int i = VA * (4 * g + r) + u;
-                S[u][v][r] = w.s_in && i < da && col + v < db ? w.in_mul * w.s_in[nh * da * db + i * w.s_i + (col + v) * w.s_j] : 0.f;
+                for (int r = 0; r < 4; r++) S[u][v][r] = entering(w, nh, VA * (4 * g + r) + u, col + v);
             }
+        }
 
     // the scores' weights (i = c, j = 4 g + r; the other block of rows is 16 further), the rows' of the carried state, and the
     // tokens' on the state after a whole chunk
@@ -173,32 +213,35 @@ __global__ __launch_bounds__(256) void k_sweep(Sweeps all) {
     const float whole = power(lg, CH);
 
     // the starts of tokens [seen, seen + 128) as two words; the third window's bytes are on their way
-    const uint8_t* flags = w.start ? w.start + n * w.start_sn : nullptr;
-    auto flag = [&](int64_t x) { return flags && x < steps && (x || w.first) ? flags[x * w.start_st] : (uint8_t)0; };
-    uint64_t m0 = 0, m1 = 0;
+    const uint8_t* flags = w.start ? w.start + n * w.start_sn + x0 * w.start_st : nullptr;
+    const bool first = w.first || seg;
+    auto flag = [&](int x) { return x < steps && (x || first) ? flags[x * w.start_st] : (uint8_t)0; };
+    uint64_t m0 = 0, m1 = 0, any = 0;
     uint8_t ahead = 0;
-    int64_t seen = 0;
+    int seen = 0;
     if (flags) {
-        m0 = __ballot(flag(lane) != 0), m1 = __ballot(flag(64 + lane) != 0);
+        uint8_t f0 = flag(lane), f1 = flag(64 + lane);
         ahead = flag(128 + lane);
+        m0 = __ballot(f0 != 0), m1 = __ballot(f1 != 0);
     }
 
-    int64_t slow = 0;  // tokens below it are taken one at a time
-    for (int64_t x = 0; x < steps;) {
-        int64_t left = steps - x;
-        int n_tok = left < CH ? (int)left : CH;
+    int slow = 0;  // tokens below it are taken one at a time
+    for (int x = 0; x < steps;) {
+        int n_tok = steps - x < CH ? steps - x : CH;
         if (flags) {
             if (x - seen >= 64) {
                 m0 = m1, m1 = __ballot(ahead != 0), seen += 64;
                 ahead = flag(seen + 128 + lane);
             }
-            int at = (int)(x - seen);
+            int at = x - seen;
             uint64_t m = at ? m0 >> at | m1 << (64 - at) : m0;
-            if (m & 1)
+            if (m & 1) {
+                any = 1;
 #pragma unroll
                 for (int u = 0; u < VA; u++)
 #pragma unroll
                     for (int v = 0; v < VB; v++) S[u][v] = (f4)0.f;
+            }
             uint64_t next = m & ~1ull;
             if (next) {
                 int d = __builtin_ctzll(next);
@@ -210,37 +253,43 @@ __global__ __launch_bounds__(256) void k_sweep(Sweeps all) {
         T ar[NB][DA / 4], br[NB][DA / 4], bt[FE][VA], ct[FE][VB];
         if (n_tok == CH) {
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                fetch<T, DA / 4, MODE>(ar[b], pa + 16 * b * sta, g * (DA / 4), da);
-                fetch<T, DA / 4, MODE>(br[b], pb + 16 * b * stb, g * (DA / 4), da);
-            }
+            for (int b = 0; b < NB; b++)
+                if (!STATE) {
+                    fetch<T, DA / 4, MODE>(ar[b], pa + 16 * b * sta, g * (DA / 4), da);
+                    fetch<T, DA / 4, MODE>(br[b], pb + 16 * b * stb, g * (DA / 4), da);
+                }
 #pragma unroll
             for (int e = 0; e < FE; e++) {
                 int64_t j = e / 4 * 16 + e % 4;
                 fetch<T, VA, MODE>(bt[e], pbt + j * stb, VA * c, da);
                 fetch<T, VB, MODE>(ct[e], pct + j * stc, col, db);
             }
-        } else {  // tokens past the chunk's end: its last one's values, replaced by zeros
+        } else {  // tokens past the chunk's end: its last one's values, replaced by zeros once all loads are on their way
+            auto over = [&](int i) { return i < n_tok ? 0 : i - n_tok + 1; };
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                int i = 16 * b + c, over = i < n_tok ? 0 : i - n_tok + 1;
-                fetch<T, DA / 4, MODE>(ar[b], pa + (16 * b - over) * sta, g * (DA / 4), da);
-                fetch<T, DA / 4, MODE>(br[b], pb + (16 * b - over) * stb, g * (DA / 4), da);
-                if (over)
-#pragma unroll
-                    for (int e = 0; e < DA / 4; e++) ar[b][e] = br[b][e] = (T)0.f;
-            }
+            for (int b = 0; b < NB; b++)
+                if (!STATE) {
+                    int64_t at = 16 * b - over(16 * b + c);
+                    fetch<T, DA / 4, MODE>(ar[b], pa + at * sta, g * (DA / 4), da);
+                    fetch<T, DA / 4, MODE>(br[b], pb + at * stb, g * (DA / 4), da);
+                }
 #pragma unroll
             for (int e = 0; e < FE; e++) {
-                int j = e / 4 * 16 + e % 4, i = j + 4 * g, over = i < n_tok ? 0 : i - n_tok + 1;
-                fetch<T, VA, MODE>(bt[e], pbt + (int64_t)(j - over) * stb, VA * c, da);
-                fetch<T, VB, MODE>(ct[e], pct + (int64_t)(j - over) * stc, col, db);
-                if (over) {
+                int j = e / 4 * 16 + e % 4;
+                int64_t at = j - over(j + 4 * g);
+                fetch<T, VA, MODE>(bt[e], pbt + at * stb, VA * c, da);
+                fetch<T, VB, MODE>(ct[e], pct + at * stc, col, db);
+            }
 #pragma unroll
-                    for (int u = 0; u < VA; u++) bt[e][u] = (T)0.f;
-#pragma unroll
-                    for (int u = 0; u < VB; u++) ct[e][u] = (T)0.f;
+            for (int b = 0; b < NB; b++)
+                if (!STATE) {
+                    unsigned mask = 16 * b + c < n_tok ? ~0u : 0u;
+                    only<T, DA / 4>(ar[b], mask), only<T, DA / 4>(br[b], mask);
                 }
+#pragma unroll
+            for (int e = 0; e < FE; e++) {
+                unsigned mask = e / 4 * 16 + e % 4 + 4 * g < n_tok ? ~0u : 0u;
+                only<T, VA>(bt[e], mask), only<T, VB>(ct[e], mask);
             }
         }
         Frag fa[NB][NF], fb[NB][NF], fbt[VA], fct[VB];
@@ -258,6 +307,7 @@ __global__ __launch_bounds__(256) void k_sweep(Sweeps all) {
             for (int u = 0; u < VB; u++) fct[u][e] = ct[e][u];
         }
 
+        if constexpr (!STATE) {
         // scores, transposed: row j = 4 g + r, column i = c
         float p[NB][FE];
 #pragma unroll
@@ -343,6 +393,8 @@ __global__ __launch_bounds__(256) void k_sweep(Sweeps all) {
                     }
                 }
 
+        }  // !STATE
+
         // the state: c weighted by its decay to the chunk's end.  In 16 bits the weighted value goes in as two parts of T, which
         // keeps the state as exact as float32 sums of this length are.  fp16 is brought to 2^14 .. 2^15 for it, where the second
         // part has its bits still, and the accumulators with it.
@@ -382,7 +434,15 @@ __global__ __launch_bounds__(256) void k_sweep(Sweeps all) {
         pa += n_tok * sta, pb += n_tok * stb, pbt += n_tok * stb, pct += n_tok * stc, po += n_tok * sto;
     }
 
-    if (!w.s_out) return;
+    if (STATE) {
+#pragma unroll
+        for (int u = 0; u < VA; u++)
+#pragma unroll
+            for (int v = 0; v < VB; v++) *held(all, item, VA * VB, u * VB + v, lane) = S[u][v];
+        if (lane == 0) all.left[item] = any ? 0.f : power(lg, steps);
+        return;
+    }
+    if (!w.s_out || seg + 1 < all.segs) return;
     bool drop = w.s_drop && w.s_drop[n * w.start_sn];
 #pragma unroll
     for (int u = 0; u < VA; u++)
@@ -391,8 +451,53 @@ __global__ __launch_bounds__(256) void k_sweep(Sweeps all) {
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 int i = VA * (4 * g + r) + u;
-                if (i < da && col + v < db) w.s_out[nh * da * db + i * w.s_i + (col + v) * w.s_j] = drop ? 0.f : w.out_mul * S[u][v][r];
+                if (i < da && col + v < db) w.s_out[(int64_t)nh * da * db + i * w.s_i + (col + v) * w.s_j] = drop ? 0.f : w.out_mul * S[u][v][r];
             }
+}
+
+// The states that the segments begin with, from what each adds: begin_0 = what enters, begin_{s+1} = left_s begin_s + added_s
+// (selected where left_s = 0, so that nothing passes a start).  A workgroup takes 32 float4s of one wave's accumulators; its 8 rows of
+// threads take a run of up to 16 segments each, all of whose loads are in flight at once, then hand on through LDS.
+constexpr int RUNS = 8, RUN = 16, MAX_SEGS = RUNS * RUN;
+
+template <int DA>
+__global__ __launch_bounds__(256) void k_join(Sweeps all) {
+    constexpr int VA = DA / 16, VB = 2, TILES = VA * VB;
+    __shared__ f4 sums[RUNS][32];
+    __shared__ float lefts[RUNS];
+    unsigned part = blockIdx.x % (2 * TILES), rest = blockIdx.x / (2 * TILES);
+    unsigned slice = rest % all.slices, role = rest / all.slices % all.count, nh = rest / all.slices / all.count;
+    const Sweep& w = all.w[role];
+    if ((int)slice * 16 * VB >= w.db) return;
+    int tile = part / 2, lane = part % 2 * 32 + threadIdx.x % 32, run = threadIdx.x / 32;
+    unsigned per = (all.segs + RUNS - 1) / RUNS, s0 = run * per;
+    auto item = [&](unsigned s) { return ((nh * all.segs + s) * all.count + role) * all.slices + slice; };
+    auto step = [](f4 x, float left, f4 add) { return left == 0.f ? add : x * left + add; };
+    f4 add[RUN];
+    float left[RUN];
+#pragma unroll
+    for (unsigned i = 0; i < RUN; i++) {
+        bool in = i < per && s0 + i < all.segs;
+        add[i] = in ? *held(all, item(s0 + i), TILES, tile, lane) : (f4)0.f;
+        left[i] = in ? all.left[item(s0 + i)] : 1.f;
+    }
+    f4 x = (f4)0.f;
+    float l = 1.f;
+#pragma unroll
+    for (int i = 0; i < RUN; i++) x = step(x, left[i], add[i]), l *= left[i];
+    sums[run][threadIdx.x % 32] = x;
+    if (threadIdx.x % 32 == 0) lefts[run] = l;
+    __syncthreads();
+    int g = lane / 16, c = lane % 16, u = tile / VB, v = tile % VB;
+#pragma unroll
+    for (int r = 0; r < 4; r++) x[r] = entering(w, nh, VA * (4 * g + r) + u, slice * 16 * VB + VB * c + v);
+    for (int i = 0; i < run; i++) x = step(x, lefts[i], sums[i][threadIdx.x % 32]);
+#pragma unroll
+    for (unsigned i = 0; i < RUN; i++)
+        if (i < per && s0 + i < all.segs) {
+            *held(all, item(s0 + i), TILES, tile, lane) = x;
+            x = step(x, left[i], add[i]);
+        }
 }
 
 // every access of the tensor falls on multiples of `elements` elements
@@ -409,10 +514,16 @@ static void launch(const Sweeps& s, hipStream_t st) {
         if (mode == EXACT && !(w.da == DA && w.db % 32 == 0 && all(unit))) mode = FOURS;
         if (mode == FOURS && !(w.da % 4 == 0 && w.db % 4 == 0 && all(4))) mode = ANY;
     }
-    unsigned grid = (unsigned)((s.items + 3) / 4);
-    if (mode == EXACT) k_sweep<T, DA, EXACT><<<grid, 256, 0, st>>>(s);
-    else if (mode == FOURS) k_sweep<T, DA, FOURS><<<grid, 256, 0, st>>>(s);
-    else k_sweep<T, DA, ANY><<<grid, 256, 0, st>>>(s);
+    unsigned grid = (s.items + 3) / 4;
+    if (s.segs > 1) {
+        if (mode == EXACT) k_sweep<T, DA, EXACT, true><<<grid, 256, 0, st>>>(s);
+        else if (mode == FOURS) k_sweep<T, DA, FOURS, true><<<grid, 256, 0, st>>>(s);
+        else k_sweep<T, DA, ANY, true><<<grid, 256, 0, st>>>(s);
+        k_join<DA><<<s.items / s.segs * (DA / 16 * 2) * 2, 256, 0, st>>>(s);
+    }
+    if (mode == EXACT) k_sweep<T, DA, EXACT, false><<<grid, 256, 0, st>>>(s);
+    else if (mode == FOURS) k_sweep<T, DA, FOURS, false><<<grid, 256, 0, st>>>(s);
+    else k_sweep<T, DA, ANY, false><<<grid, 256, 0, st>>>(s);
 }
 
 template <typename T>
@@ -422,16 +533,34 @@ static void launch(const Sweeps& s, hipStream_t st) {
     else launch<T, 128>(s, st);
 }
 
-// runs `count` sweeps over the same tokens; their a and b fall into one tile width
-static void launch(const urgym_ops_seq* q, const Sweep* w, int count, hipStream_t st) {
+static int tile(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+
+// The launch of `count` sweeps whose a and b fall into one tile width.  With fewer waves than fill the chip twice over (one a SIMD is
+// half of that) the axis is cut into segments, at least 64 steps each: their states are computed first, then joined.
+static Sweeps plan(const urgym_ops_seq* q, const Sweep* w, int count) {
     Sweeps s = {};
     s.count = count, s.heads = q->heads, s.steps = q->steps, s.log_decay = q->log_decay;
     for (int i = 0; i < count; i++) {
         s.w[i] = w[i];
-        int n = (w[i].db + 31) / 32;
+        unsigned n = (w[i].db + 31) / 32;
         s.slices = n > s.slices ? n : s.slices;
     }
-    s.items = q->envs * q->heads * s.count * s.slices;
+    s.items = (unsigned)(q->envs * q->heads) * s.count * s.slices;
+    int64_t segs = s.items >= 1024 ? 1 : 2048 / s.items, most = q->steps / 64;
+    segs = segs < most ? segs : most;
+    segs = segs < MAX_SEGS ? segs : MAX_SEGS;
+    if (segs < 2) segs = 1;
+    int64_t len = (q->steps + segs - 1) / segs;
+    len = (len + 31) / 32 * 32;
+    s.segs = (unsigned)((q->steps + len - 1) / len), s.seg_len = (int)len;
+    s.items *= s.segs;
+    return s;
+}
+
+static int64_t workspace(const Sweeps& s) { return s.segs > 1 ? (int64_t)s.items * (tile(s.w[0].da) * 32 + 1) : 0; }
+
+static void launch(const urgym_ops_seq* q, Sweeps s, float* ws, hipStream_t st) {
+    s.ws = ws, s.left = ws + (int64_t)s.items * tile(s.w[0].da) * 32;
     if (q->dtype == URGYM_OPS_F32) launch<float>(s, st);
     else if (q->dtype == URGYM_OPS_BF16) launch<bf16>(s, st);
     else launch<f16>(s, st);
@@ -506,33 +635,60 @@ static Sweep backward(const urgym_ops_seq* s, Rows a, Rows b, Rows c, Rows o, in
     return w;
 }
 
-static int tile(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
-
-extern "C" int64_t urgym_ops_decay_workspace(const urgym_ops_seq*, int) { return 0; }
-
-extern "C" int urgym_ops_decay(const urgym_ops_seq* s, void* o, float* state_out, float*, void* stream) {
-    if (seq_check("urgym_ops_decay", s)) return -1;
-    if (!o || !state_out) return uo_fail("urgym_ops_decay: o and state_out are needed");
-    Sweep w = forward(s, rows(s->q, s->q_stride), rows(s->k, s->k_stride), rows(s->v, s->v_stride), packed(o, s, s->dv), s->dk, s->dv, false);
-    w.s_out = state_out;
-    launch(s, &w, 1, (hipStream_t)stream);
-    return uo_launched("urgym_ops_decay");
+// the launches of one direction: o's, or those of dk, dq and dv, which read the same rows and share a launch where their tiles agree
+static int plans(const urgym_ops_seq* s, Rows o, Sweeps* p) {
+    Sweep w = forward(s, rows(s->q, s->q_stride), rows(s->k, s->k_stride), rows(s->v, s->v_stride), o, s->dk, s->dv, false);
+    p[0] = plan(s, &w, 1);
+    return 1;
 }
 
-extern "C" int urgym_ops_decay_backward(const urgym_ops_seq* s, const void* d_out, const int64_t d_out_stride[3],
-                                        const float* d_state_out, void* dq, void* dk, void* dv, float* d_state, float*,
-                                        void* stream) {
-    if (seq_check("urgym_ops_decay_backward", s)) return -1;
-    if (!d_out || !d_out_stride || !dq || !dk || !dv) return uo_fail("urgym_ops_decay_backward: d_out, dq, dk and dv are needed");
-    Rows q = rows(s->q, s->q_stride), k = rows(s->k, s->k_stride), v = rows(s->v, s->v_stride), g = rows(d_out, d_out_stride);
+static int plans(const urgym_ops_seq* s, Rows g, const float* d_state_out, void* dq, void* dk, void* dv, float* d_state, Sweeps* p) {
+    Rows q = rows(s->q, s->q_stride), k = rows(s->k, s->k_stride), v = rows(s->v, s->v_stride);
     Sweep w[3] = {backward(s, v, g, q, packed(dk, s, s->dk), s->dv, s->dk, true, d_state_out),
                   forward(s, g, v, k, packed(dq, s, s->dk), s->dv, s->dk, true),
                   backward(s, k, q, g, packed(dv, s, s->dv), s->dk, s->dv, false, d_state_out)};
     w[2].s_out = d_state;
-    hipStream_t st = (hipStream_t)stream;
-    if (tile(s->dk) == tile(s->dv)) launch(s, w, 3, st);  // one launch: the three read the same rows
-    else launch(s, w, 2, st), launch(s, w + 2, 1, st);
-    return uo_launched("urgym_ops_decay_backward");
+    if (tile(s->dk) == tile(s->dv)) {
+        p[0] = plan(s, w, 3);
+        return 1;
+    }
+    p[0] = plan(s, w, 2), p[1] = plan(s, w + 2, 1);
+    return 2;
+}
+
+extern "C" int64_t urgym_ops_decay_workspace(const urgym_ops_seq* s, int backward) {
+    if (seq_check("urgym_ops_decay_workspace", s)) return -1;
+    Sweeps p[2];
+    int64_t most = 0;
+    for (int i = 0, n = backward ? plans(s, Rows{}, nullptr, nullptr, nullptr, nullptr, nullptr, p) : plans(s, Rows{}, p); i < n; i++)
+        most = workspace(p[i]) > most ? workspace(p[i]) : most;
+    return most;
+}
+
+static int run(const char* what, const urgym_ops_seq* s, const Sweeps* p, int n, float* ws, hipStream_t st) {
+    for (int i = 0; i < n; i++)
+        if (workspace(p[i]) && !ws) return uo_fail("%s: a workspace is needed", what);
+    for (int i = 0; i < n; i++) launch(s, p[i], ws, st);
+    return uo_launched(what);
+}
+
+extern "C" int urgym_ops_decay(const urgym_ops_seq* s, void* o, float* state_out, float* ws, void* stream) {
+    if (seq_check("urgym_ops_decay", s)) return -1;
+    if (!o || !state_out) return uo_fail("urgym_ops_decay: o and state_out are needed");
+    Sweeps p[1];
+    int n = plans(s, packed(o, s, s->dv), p);
+    p[0].w[0].s_out = state_out;
+    return run("urgym_ops_decay", s, p, n, ws, (hipStream_t)stream);
+}
+
+extern "C" int urgym_ops_decay_backward(const urgym_ops_seq* s, const void* d_out, const int64_t d_out_stride[3],
+                                        const float* d_state_out, void* dq, void* dk, void* dv, float* d_state, float* ws,
+                                        void* stream) {
+    if (seq_check("urgym_ops_decay_backward", s)) return -1;
+    if (!d_out || !d_out_stride || !dq || !dk || !dv) return uo_fail("urgym_ops_decay_backward: d_out, dq, dk and dv are needed");
+    Sweeps p[2];
+    int n = plans(s, rows(d_out, d_out_stride), d_state_out, dq, dk, dv, d_state, p);
+    return run("urgym_ops_decay_backward", s, p, n, ws, (hipStream_t)stream);
 }
 
 extern "C" int urgym_ops_decay_step(int dtype, int64_t envs, int heads, int dk, int dv, const void* q, int64_t q_sn, int64_t q_sh,
