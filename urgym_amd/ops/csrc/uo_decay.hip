@@ -14,18 +14,24 @@
 // which are matrix products.  A chunk ends where the next episode begins, so every chunk lies in one episode and the only mask
 // is i >= j; rows past its end are zeroed by selection, so that nothing of another episode, a NaN included, is ever multiplied.
 //
-// One wave holds 32 columns of one (env, head)'s C in the accumulators of 16x16 matrix instructions for the whole sweep and
-// needs no LDS and no barrier, because the operands' layouts meet in registers (c = lane % 16, g = lane / 16):
+// One wave (a workgroup of its own: no barrier) holds 16 VB columns of one (env, head)'s C in the accumulators of 16x16 matrix
+// instructions for the whole sweep.  While a chunk is computed with, the next one's rows are on their way from memory into the
+// other half of the wave's LDS, without passing through registers.  The operands' layouts meet (c = lane % 16, g = lane / 16):
 //   * an accumulator holds rows 4 g + r of column c; as the next product's operand its lane holds 4 elements of the contracted
-//     axis at 4 g + r.  The order of a contracted axis is free as long as both sides share it, so scores (b a^T, transposed) feed
-//     the product with c, and C the product with a, after a conversion only;
-//   * row 4 g + r of C's tile u is dimension VA (4 g + r) + u: a lane's part of a row of a or b is then contiguous, and
-//     the transposed operands (tokens contracted) are loaded as VA or VB neighbouring columns of one token per lane.
+//     axis at 4 g + r.  Scores (b a^T, transposed) feed the product with c, and C the product with a, after a conversion only;
+//   * o is computed transposed, so that a lane holds neighbouring columns of one token, which it stores as a vector;
+//   * 16-bit operands that contract the tokens are transposed on their way out of LDS.
+// LDS rows are swizzled in units of 32 bytes, so that both kinds of reads spread over the banks.
 #include "uo_common.h"
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <int N>
+struct Int {
+    static constexpr int value = N;
+};
 
 struct Rows {  // one tensor [steps, envs, heads, d]
     const void* p;
@@ -59,22 +65,40 @@ struct Sweeps {
 };
 
 template <typename T>
-struct Kind;
-template <>
-struct Kind<float> {
-    typedef f4 Frag;
-    static constexpr int FE = 4;
+struct Kind {
+    static constexpr bool HALF = sizeof(T) == 2, F16 = __is_same(T, f16);
+};
+template <typename T>
+struct FragOf {
+    typedef f4 type;
 };
 template <>
-struct Kind<bf16> {
-    typedef bf16x8 Frag;
-    static constexpr int FE = 8;
+struct FragOf<bf16> {
+    typedef bf16x8 type;
 };
 template <>
-struct Kind<f16> {
-    typedef f16x8 Frag;
-    static constexpr int FE = 8;
+struct FragOf<f16> {
+    typedef f16x8 type;
 };
+
+// A wave's tiles: CH tokens of a and b (DA wide) and of 16 VB columns of c, in LDS twice
+template <typename T, int DA_, int VB_>
+struct Tile {
+    static constexpr int DA = DA_, VB = VB_, ES = sizeof(T), FE = 16 / ES, NB = FE / 4, CH = 16 * NB, NF = DA / 4 / FE, VA = DA / 16;
+    static constexpr int RA = DA * ES, RC = 16 * VB * ES;  // bytes of a row
+    static constexpr int A0 = 0, B0 = CH * RA, C0 = 2 * CH * RA, BUF = 2 * CH * RA + CH * RC;
+    // the dimension of row m of C's tile u, and the column (of the wave's) of its column m of tile v
+    static __device__ __forceinline__ int dim(int u, int m) { return ES == 2 ? 16 * u + m : VA * m + u; }
+    static __device__ __forceinline__ int col(int v, int m) { return ES == 2 ? 32 * (v / 2) + 8 * (m / 4) + 4 * (v % 2) + m % 4 : VB * m + v; }
+};
+
+// where byte `byte` of row t lies in a tile of RB bytes a row: 32-byte units, exchanged so that 8 neighbouring units of one column
+// of units (8 rows at least) fall on 256 different bytes
+template <int RB>
+__device__ __forceinline__ int place(int t, int byte) {
+    constexpr int U = RB / 32, R = U >= 8 ? 1 : 8 / U;
+    return t * RB + ((byte / 32 ^ t / R % U) * 32) + byte % 32;
+}
 
 // acc += a b over the fragments' contracted axis (32 deep in 16 bits, 4 x 4 in 32)
 __device__ __forceinline__ f4 dot(f4 acc, bf16x8 a, bf16x8 b) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0); }
@@ -87,43 +111,88 @@ __device__ __forceinline__ f4 dot(f4 acc, f4 a, f4 b) {
 
 __device__ __forceinline__ float power(float lg, int n) { return n == 0 ? 1.f : exp2f(lg * (float)n); }
 
-// How a row's elements are fetched: EXACT: the width is the tile's and everything is 16-byte aligned; FOURS: the width and every
-// offset are multiples of 4 elements; ANY: one element at a time.
+// How rows are fetched.  EXACT: widths are the tiles' and everything is 16-byte aligned: from memory into LDS directly.  Otherwise
+// through registers, 4 elements at a time where widths and offsets are multiples of 4 (FOURS), or one (ANY).
 enum { EXACT, FOURS, ANY };
 
-// N elements (a power of two) at p, of which those from column col on that are below width exist
-template <typename T, int N, int MODE>
-__device__ __forceinline__ void fetch(T* to, const T* p, int col, int width) {
-    constexpr int U = MODE == ANY ? 1 : MODE == FOURS ? (N < 4 ? N : 4) : (N * (int)sizeof(T) <= 16 ? N : 16 / (int)sizeof(T));
-    typedef T V __attribute__((ext_vector_type(U)));
+// 16 bytes of elements at p as words; of those from column col on, the ones below width exist
+template <typename T, int MODE>
+__device__ __forceinline__ void fetch(unsigned* to, const T* p, int col, int width) {
+    if constexpr (MODE == FOURS) {
+        typedef unsigned V __attribute__((ext_vector_type(sizeof(T))));
 #pragma unroll
-    for (int u = 0; u < N; u += U) {
-        if constexpr (U == 1) {
-            to[u] = MODE == EXACT || col + u < width ? p[u] : (T)0.f;
-        } else {
-            V x = (V)(T)0.f;
-            if (MODE == EXACT || col + u < width) x = *(const V*)(p + u);
+        for (int i = 0; i < 4; i += sizeof(T)) {
+            V x = (V)0u;
+            if (col + i * 4 / (int)sizeof(T) < width) x = *(const V*)((const unsigned*)p + i);
 #pragma unroll
-            for (int e = 0; e < U; e++) to[u + e] = x[e];
+            for (int e = 0; e < (int)sizeof(T); e++) to[i + e] = x[e];
+        }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) to[i] = col + i < width ? ((const unsigned*)p)[i] : 0u;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            unsigned lo = col + 2 * i < width ? ((const uint16_t*)p)[2 * i] : 0u;
+            to[i] = lo | (col + 2 * i + 1 < width ? (unsigned)((const uint16_t*)p)[2 * i + 1] << 16 : 0u);
         }
     }
 }
 
-// N elements, or zeros where the mask is zero (a selection: nothing of what is dropped is computed with)
-template <typename T, int N>
-__device__ __forceinline__ void only(T* x, unsigned mask) {
-    constexpr int U = 4 / sizeof(T);
-    typedef T V __attribute__((ext_vector_type(U)));
+// 16 bytes of each lane's address to LDS bytes to .. to + 1023, lane by lane.  Written as assembly because the compiler would wait
+// for it before the next read of LDS, whichever half that reads; the waits are `landed`.  (m0, the address in LDS, has no other
+// use in these kernels.)
+__device__ __forceinline__ void load_to_lds(unsigned to, const void* from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+}
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// N words, or zeros where the mask is zero (a selection: nothing of what is dropped is computed with)
+template <int N>
+__device__ __forceinline__ void only(unsigned* x, unsigned mask) {
 #pragma unroll
-    for (int i = 0; i < N; i += U) {
-        if constexpr (U == 1) {
-            x[i] = __uint_as_float(__float_as_uint(x[i]) & mask);
-        } else {
-            V v;
-            v[0] = x[i], v[1] = x[i + 1];
-            v = __builtin_bit_cast(V, __builtin_bit_cast(unsigned, v) & mask);
-            x[i] = v[0], x[i + 1] = v[1];
+    for (int i = 0; i < N; i++) x[i] &= mask;
+}
+
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+
+// Fragments from LDS, as words.  `row`: row t of a tile, the f-th part of it (operand with the dimensions contracted);
+// `column`: tile u of its columns with the tokens contracted (DIM: a's and b's dimensions, else c's columns).
+template <class L, int RB>
+__device__ __forceinline__ u4 row(const char* tile, int t, int f, int g) {
+    if constexpr (L::ES == 2) {
+        u2 lo = *(const u2*)(tile + place<RB>(t, 64 * f + 8 * g)), hi = *(const u2*)(tile + place<RB>(t, 64 * f + 32 + 8 * g));
+        return u4{lo[0], lo[1], hi[0], hi[1]};
+    } else {
+        return *(const u4*)(tile + place<RB>(t, g * (RB / 4) + 16 * f));
+    }
+}
+
+template <class L, int RB, bool DIM, int N>
+__device__ __forceinline__ void columns(u4* to, const char* tile, int c, int g) {
+    if constexpr (L::ES == 2) {
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s4* P;
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            int byte = DIM ? 32 * u + 8 * (c % 4) : 64 * (u / 2) + 16 * (c % 4) + 8 * (u % 2);
+            const char* at = tile + place<RB>(4 * g + c / 4, byte);
+            u2 lo = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at)));
+            u2 hi = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at + 16 * RB)));
+            to[u] = u4{lo[0], lo[1], hi[0], hi[1]};
         }
+    } else {
+        constexpr int W = N < 4 ? N : 4;
+        typedef unsigned V __attribute__((ext_vector_type(W)));
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int u = 0; u < N; u += W) {
+                V x = *(const V*)(tile + place<RB>(4 * g + r, (N * c + u) * 4));
+#pragma unroll
+                for (int e = 0; e < W; e++) to[u + e][r] = x[e];
+            }
     }
 }
 
@@ -153,33 +222,32 @@ __device__ __forceinline__ f4* held(const Sweeps& all, unsigned item, int tiles,
 }
 
 // STATE: only what the segment adds to the state (no a, no o); segments after it need that before they can begin.
-template <typename T, int DA, int MODE, bool STATE>
-__global__ __launch_bounds__(256) void k_sweep(Sweeps all) {
-    typedef typename Kind<T>::Frag Frag;
-    constexpr int FE = Kind<T>::FE, NB = FE / 4, CH = 16 * NB, NF = DA / 4 / FE, VA = DA / 16, VB = 2;
-    constexpr bool HALF = sizeof(T) == 2, F16 = HALF && T(1.0 / 1024 + 1) != T(1);
-    unsigned item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / UO_WAVE);
+template <typename T, class L, int MODE, bool STATE>
+__global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
+    typedef typename FragOf<T>::type Frag;
+    constexpr int FE = L::FE, NB = L::NB, CH = L::CH, NF = L::NF, VA = L::VA, VB = L::VB, RA = L::RA, RC = L::RC;
+    constexpr bool HALF = Kind<T>::HALF, F16 = Kind<T>::F16;
+    __shared__ __attribute__((aligned(256))) char lds[2 * L::BUF];
+    // workgroups go to the 8 XCDs in turn: each takes a run of items, for neighbours share rows -- the slices, then the sweeps,
+    // then the heads of one env -- and their L2
+    unsigned item = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
     if (item >= all.items) return;
-    // neighbours share their rows: the slices, then the sweeps, then the heads of one env
     unsigned slice = item % all.slices, rest = item / all.slices, role = rest % all.count, nhs = rest / all.count;
     unsigned nh = nhs / all.segs, seg = nhs % all.segs, h = nh % all.heads;
     int64_t n = nh / all.heads;
-    int lane = threadIdx.x % UO_WAVE, c = lane % 16, g = lane / 16;
+    const int lane = threadIdx.x, c = lane % 16, g = lane / 16;
     const Sweep& w = all.w[role];
-    int j0 = slice * 16 * VB;
-    if (j0 >= w.db) return;
-    const int col = j0 + VB * c, da = w.da, db = w.db;
+    const int j0 = slice * 16 * VB, da = w.da, db = w.db;
+    if (j0 >= db) return;
     const int64_t x0 = (int64_t)seg * all.seg_len, left_steps = all.steps - x0;
     const int steps = left_steps < all.seg_len ? (int)left_steps : all.seg_len;
-    float lg = all.log_decay[h] * 1.44269504088896340736f;
-
-    // lane pointers: a row's part (token c), and neighbouring columns of token 4 g
-    const T* pa = (const T*)w.a.p + n * w.a.sn + h * w.a.sh + (x0 + c) * w.a.st + g * (DA / 4);
-    const T* pb = (const T*)w.b.p + n * w.b.sn + h * w.b.sh + (x0 + c) * w.b.st + g * (DA / 4);
-    const T* pbt = (const T*)w.b.p + n * w.b.sn + h * w.b.sh + (x0 + 4 * g) * w.b.st + VA * c;
-    const T* pct = (const T*)w.c.p + n * w.c.sn + h * w.c.sh + (x0 + 4 * g) * w.c.st + col;
-    T* po = (T*)w.o.p + n * w.o.sn + h * w.o.sh + (x0 + 4 * g) * w.o.st + col;
+    const float lg = all.log_decay[h] * 1.44269504088896340736f;
+    const T* const pa = (const T*)w.a.p + n * w.a.sn + h * w.a.sh + x0 * w.a.st;
+    const T* const pb = (const T*)w.b.p + n * w.b.sn + h * w.b.sh + x0 * w.b.st;
+    const T* const pc = (const T*)w.c.p + n * w.c.sn + h * w.c.sh + x0 * w.c.st + j0;
     const int64_t sta = w.a.st, stb = w.b.st, stc = w.c.st, sto = w.o.st;
+    // o: token c, the lane's run of 4 VB columns (float32) or its runs of 8 (16 bits: one in every 32)
+    T* const po = (T*)w.o.p + n * w.o.sn + h * w.o.sh + (x0 + c) * sto + j0 + (HALF ? 8 : 4 * VB) * g;
 
     f4 S[VA][VB];
 #pragma unroll
@@ -192,24 +260,23 @@ __global__ __launch_bounds__(256) void k_sweep(Sweeps all) {
                 S[u][v] = *held(all, item, VA * VB, u * VB + v, lane);
             } else {
 #pragma unroll
-                for (int r = 0; r < 4; r++) S[u][v][r] = entering(w, nh, VA * (4 * g + r) + u, col + v);
+                for (int r = 0; r < 4; r++) S[u][v][r] = entering(w, nh, L::dim(u, 4 * g + r), j0 + L::col(v, c));
             }
         }
 
     // the scores' weights (i = c, j = 4 g + r; the other block of rows is 16 further), the rows' of the carried state, and the
     // tokens' on the state after a whole chunk
-    float near[4], far[4], carry[NB][4], enter[FE];
+    float near[4], far[4], carry[NB], enter[FE];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
         int d = c - 4 * g - r;
         near[r] = d >= 0 ? w.sa * w.sb * power(lg, d) : 0.f;
         far[r] = w.sa * w.sb * power(lg, 16 + d);
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            carry[b][r] = w.sa * power(lg, 16 * b + 4 * g + r + w.e0);
-            enter[4 * b + r] = w.sb * power(lg, CH - (16 * b + 4 * g + r) - w.e0);
-        }
+        for (int b = 0; b < NB; b++) enter[4 * b + r] = w.sb * power(lg, CH - (16 * b + 4 * g + r) - w.e0);
     }
+#pragma unroll
+    for (int b = 0; b < NB; b++) carry[b] = w.sa * power(lg, 16 * b + c + w.e0);
     const float whole = power(lg, CH);
 
     // the starts of tokens [seen, seen + 128) as two words; the third window's bytes are on their way
@@ -226,174 +293,193 @@ __global__ __launch_bounds__(256) void k_sweep(Sweeps all) {
     }
 
     int slow = 0;  // tokens below it are taken one at a time
-    for (int x = 0; x < steps;) {
+    // the chunk that begins at token x: its length, and whether an episode begins with it
+    auto chunk = [&](int x, bool* fresh) {
         int n_tok = steps - x < CH ? steps - x : CH;
+        *fresh = false;
         if (flags) {
-            if (x - seen >= 64) {
-                m0 = m1, m1 = __ballot(ahead != 0), seen += 64;
-                ahead = flag(seen + 128 + lane);
-            }
             int at = x - seen;
-            uint64_t m = at ? m0 >> at | m1 << (64 - at) : m0;
-            if (m & 1) {
-                any = 1;
-#pragma unroll
-                for (int u = 0; u < VA; u++)
-#pragma unroll
-                    for (int v = 0; v < VB; v++) S[u][v] = (f4)0.f;
-            }
+            uint64_t m = at == 0 ? m0 : at < 64 ? m0 >> at | m1 << (64 - at) : m1 >> (at - 64);
+            *fresh = m & 1;
             uint64_t next = m & ~1ull;
             if (next) {
                 int d = __builtin_ctzll(next);
                 n_tok = d < n_tok ? d : n_tok;
             }
         }
-        if (x < slow) n_tok = 1;
+        return x < slow ? 1 : n_tok;
+    };
 
-        T ar[NB][DA / 4], br[NB][DA / 4], bt[FE][VA], ct[FE][VB];
-        if (n_tok == CH) {
+    // A chunk's rows into one half of LDS: `issue`, then (loads that pass through registers) `commit`, then `landed`.  Lane by lane
+    // 16 bytes; rows past the chunk's end are its last one's, zeroed before they are used.
+    constexpr int KA = CH * RA / 1024, KC = CH * RC / 1024;
+    unsigned stage[MODE == EXACT ? 1 : 2 * KA + KC][4];
+    const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    auto rows_of = [&](auto size, auto part, int k0, const T* base, int64_t st, int tile0, int width, int n_tok, int buf) {
+        constexpr int RB = decltype(size)::value, K = decltype(part)::value;
 #pragma unroll
-            for (int b = 0; b < NB; b++)
-                if (!STATE) {
-                    fetch<T, DA / 4, MODE>(ar[b], pa + 16 * b * sta, g * (DA / 4), da);
-                    fetch<T, DA / 4, MODE>(br[b], pb + 16 * b * stb, g * (DA / 4), da);
-                }
-#pragma unroll
-            for (int e = 0; e < FE; e++) {
-                int64_t j = e / 4 * 16 + e % 4;
-                fetch<T, VA, MODE>(bt[e], pbt + j * stb, VA * c, da);
-                fetch<T, VB, MODE>(ct[e], pct + j * stc, col, db);
-            }
-        } else {  // tokens past the chunk's end: its last one's values, replaced by zeros once all loads are on their way
-            auto over = [&](int i) { return i < n_tok ? 0 : i - n_tok + 1; };
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-                if (!STATE) {
-                    int64_t at = 16 * b - over(16 * b + c);
-                    fetch<T, DA / 4, MODE>(ar[b], pa + at * sta, g * (DA / 4), da);
-                    fetch<T, DA / 4, MODE>(br[b], pb + at * stb, g * (DA / 4), da);
-                }
-#pragma unroll
-            for (int e = 0; e < FE; e++) {
-                int j = e / 4 * 16 + e % 4;
-                int64_t at = j - over(j + 4 * g);
-                fetch<T, VA, MODE>(bt[e], pbt + at * stb, VA * c, da);
-                fetch<T, VB, MODE>(ct[e], pct + at * stc, col, db);
-            }
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-                if (!STATE) {
-                    unsigned mask = 16 * b + c < n_tok ? ~0u : 0u;
-                    only<T, DA / 4>(ar[b], mask), only<T, DA / 4>(br[b], mask);
-                }
-#pragma unroll
-            for (int e = 0; e < FE; e++) {
-                unsigned mask = e / 4 * 16 + e % 4 + 4 * g < n_tok ? ~0u : 0u;
-                only<T, VA>(bt[e], mask), only<T, VB>(ct[e], mask);
-            }
+        for (int k = 0; k < K; k++) {
+            int t = k * (1024 / RB) + lane / (RB / 16);
+            int byte = place<RB>(t, lane * 16 % RB) - t * RB;  // exchanging units twice is nothing: what belongs at this place
+            int64_t tt = n_tok == CH || t < n_tok ? t : n_tok - 1;
+            const T* from = base + tt * st + byte / (int)sizeof(T);
+            if constexpr (MODE == EXACT) load_to_lds(__builtin_amdgcn_readfirstlane(at + buf * L::BUF + tile0 + k * 1024), from);
+            else fetch<T, MODE>(stage[k0 + k], from, byte / (int)sizeof(T), width);
         }
-        Frag fa[NB][NF], fb[NB][NF], fbt[VA], fct[VB];
+    };
+    auto issue = [&](int buf, int x, int n_tok) {
+        if (MODE == EXACT) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every read of this half has been answered
+        if (!STATE) rows_of(Int<RA>(), Int<KA>(), 0, pa + x * sta, sta, L::A0, da, n_tok, buf);
+        rows_of(Int<RA>(), Int<KA>(), KA, pb + x * stb, stb, L::B0, da, n_tok, buf);
+        rows_of(Int<RC>(), Int<KC>(), 2 * KA, pc + x * stc, stc, L::C0, db - j0, n_tok, buf);
+    };
+    auto commit = [&](int buf) {
+        if constexpr (MODE == EXACT) landed();
+        else
 #pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int f = 0; f < NF; f++)
-#pragma unroll
-                for (int e = 0; e < FE; e++) fa[b][f][e] = ar[b][f * FE + e], fb[b][f][e] = br[b][f * FE + e];
-#pragma unroll
-        for (int e = 0; e < FE; e++) {
-#pragma unroll
-            for (int u = 0; u < VA; u++) fbt[u][e] = bt[e][u];
-#pragma unroll
-            for (int u = 0; u < VB; u++) fct[u][e] = ct[e][u];
-        }
+            for (int k = STATE ? KA : 0; k < 2 * KA + KC; k++)
+                *(u4*)(lds + buf * L::BUF + k * 1024 + lane * 16) = u4{stage[k][0], stage[k][1], stage[k][2], stage[k][3]};
+    };
 
-        if constexpr (!STATE) {
-        // scores, transposed: row j = 4 g + r, column i = c
-        float p[NB][FE];
-#pragma unroll
-        for (int it = 0; it < NB; it++)
-#pragma unroll
-            for (int jb = 0; jb < NB; jb++) {
-                f4 acc = (f4)0.f;
-                if (jb <= it)
-#pragma unroll
-                    for (int f = 0; f < NF; f++) acc = dot(acc, fb[jb][f], fa[it][f]);
-#pragma unroll
-                for (int r = 0; r < 4; r++) p[it][4 * jb + r] = jb < it ? acc[r] * far[r] : jb == it ? (c >= 4 * g + r ? acc[r] * near[r] : 0.f) : 0.f;
-            }
-        float p_down = 1.f, p_up = 1.f, s_down = 1.f, s_up = 1.f;
-        if constexpr (F16) {
-            float most = 0.f;
-#pragma unroll
-            for (int it = 0; it < NB; it++)
-#pragma unroll
-                for (int e = 0; e < FE; e++) most = fmaxf(most, fabsf(p[it][e]));
-            unit(wave_max(most), &p_down, &p_up);
-            most = 0.f;
+    // One chunk from LDS: o, then the state; `then` runs in between, before o is stored.  False (and nothing done) where the chunk
+    // has to be taken token by token.
+    auto compute = [&](auto half, int x, int n_tok, bool fresh, auto then) {
+        const char* buf = lds + decltype(half)::value * L::BUF;
+        if (fresh) {
+            any = 1;
 #pragma unroll
             for (int u = 0; u < VA; u++)
 #pragma unroll
-                for (int v = 0; v < VB; v++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) most = fmaxf(most, fabsf(S[u][v][r]));
-            unit(wave_max(most), &s_down, &s_up);
+                for (int v = 0; v < VB; v++) S[u][v] = (f4)0.f;
         }
-
-        // o: the carried state's part, weighted by row, then the chunk's own.  Scores and state are rounded to T here: an error of
-        // half a step of T in each product, as large as that of the output's own rounding.
-        f4 O[NB][VB];
+        u4 wct[VB];
+        columns<L, RC, false, VB>(wct, buf + L::C0, c, g);
+        u4 tokens = (u4)~0u;  // which of an operand's tokens exist
+        if (n_tok < CH) {
 #pragma unroll
-        for (int v = 0; v < VB; v++) {
-            Frag fs[NF];
-#pragma unroll
-            for (int e = 0; e < DA / 4; e++) fs[e / FE][e % FE] = (T)(F16 ? S[e % VA][v][e / VA] * s_down : S[e % VA][v][e / VA]);
-#pragma unroll
-            for (int it = 0; it < NB; it++) {
-                f4 acc = (f4)0.f;
-#pragma unroll
-                for (int f = 0; f < NF; f++) acc = dot(acc, fa[it][f], fs[f]);
-#pragma unroll
-                for (int r = 0; r < 4; r++) acc[r] *= F16 ? carry[it][r] * (s_up * p_down) : carry[it][r];
-                Frag fp;
-#pragma unroll
-                for (int e = 0; e < FE; e++) fp[e] = (T)(F16 ? p[it][e] * p_down : p[it][e]);
-                O[it][v] = dot(acc, fp, fct[v]);
+            for (int i = 0; i < 4; i++) {
+                if (HALF) {
+                    int t = 16 * (i / 2) + 4 * g + 2 * (i % 2);
+                    tokens[i] = (t < n_tok ? 0xffffu : 0u) | (t + 1 < n_tok ? 0xffff0000u : 0u);
+                } else {
+                    tokens[i] = 4 * g + i < n_tok ? ~0u : 0u;
+                }
             }
+#pragma unroll
+            for (int v = 0; v < VB; v++) wct[v] &= tokens;
         }
-        // A zero score times an infinity or NaN of a later token is NaN: such a chunk is done again token by token.
-        if (n_tok > 1) {
-            float z = 0.f;
+        Frag fct[VB];
+#pragma unroll
+        for (int v = 0; v < VB; v++) fct[v] = __builtin_bit_cast(Frag, wct[v]);
+
+        if constexpr (!STATE) {
+            // scores, transposed: row j = 4 g + r, column i = c
+            Frag fa[NB][NF];
+            f4 sc[NB][NB];
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int f = 0; f < NF; f++) {
+                    u4 wa = row<L, RA>(buf + L::A0, 16 * b + c, f, g);
+                    if (n_tok < CH) wa &= 16 * b + c < n_tok ? ~0u : 0u;
+                    fa[b][f] = __builtin_bit_cast(Frag, wa);
+                }
+#pragma unroll
+            for (int jb = 0; jb < NB; jb++)
+#pragma unroll
+                for (int f = 0; f < NF; f++) {
+                    u4 wb = row<L, RA>(buf + L::B0, 16 * jb + c, f, g);
+                    if (n_tok < CH) wb &= 16 * jb + c < n_tok ? ~0u : 0u;
+#pragma unroll
+                    for (int it = jb; it < NB; it++) sc[it][jb] = dot(f ? sc[it][jb] : (f4)0.f, __builtin_bit_cast(Frag, wb), fa[it][f]);
+                }
+            float p[NB][FE];
 #pragma unroll
             for (int it = 0; it < NB; it++)
 #pragma unroll
-                for (int v = 0; v < VB; v++)
+                for (int jb = 0; jb < NB; jb++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) z += O[it][v][r] * 0.f;
-            if (__any(z != z)) {
-                slow = x + n_tok;
-                continue;
+                    for (int r = 0; r < 4; r++) p[it][4 * jb + r] = jb < it ? sc[it][jb][r] * far[r] : jb == it ? sc[it][jb][r] * near[r] : 0.f;
+            float p_down = 1.f, p_up = 1.f, s_down = 1.f, s_up = 1.f;
+            if constexpr (F16) {
+                float most = 0.f;
+#pragma unroll
+                for (int it = 0; it < NB; it++)
+#pragma unroll
+                    for (int e = 0; e < FE; e++) most = fmaxf(most, fabsf(p[it][e]));
+                unit(wave_max(most), &p_down, &p_up);
+                most = 0.f;
+#pragma unroll
+                for (int u = 0; u < VA; u++)
+#pragma unroll
+                    for (int v = 0; v < VB; v++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) most = fmaxf(most, fabsf(S[u][v][r]));
+                unit(wave_max(most), &s_down, &s_up);
             }
-        }
+
+            // o, transposed: the carried state's part, weighted by token, then the chunk's own.  Scores and state are rounded to T
+            // here: an error of half a step of T in each product, as large as that of the output's own rounding.
+            f4 O[NB][VB];
+            Frag fp[NB];
 #pragma unroll
-        for (int it = 0; it < NB; it++)
+            for (int it = 0; it < NB; it++)
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-                if (16 * it + 4 * g + r < n_tok) {
-                    T* to = po + (int64_t)(16 * it + r) * sto;
-                    if (MODE != ANY) {
-                        typedef T V __attribute__((ext_vector_type(VB)));
-                        V y;
+                for (int e = 0; e < FE; e++) fp[it][e] = (T)(F16 ? p[it][e] * p_down : p[it][e]);
 #pragma unroll
-                        for (int v = 0; v < VB; v++) y[v] = (T)(F16 ? O[it][v][r] * p_up : O[it][v][r]);
-                        if (MODE == EXACT || col < db) *(V*)to = y;
-                    } else {
+            for (int v = 0; v < VB; v++) {
+                Frag fs[NF];
 #pragma unroll
-                        for (int v = 0; v < VB; v++)
-                            if (col + v < db) to[v] = (T)(F16 ? O[it][v][r] * p_up : O[it][v][r]);
+                for (int i = 0; i < L::DA / 4; i++) {
+                    int u = HALF ? i / 4 : i % VA, r = HALF ? i % 4 : i / VA;
+                    fs[i / FE][i % FE] = (T)(F16 ? S[u][v][r] * s_down : S[u][v][r]);
+                }
+#pragma unroll
+                for (int it = 0; it < NB; it++) {
+                    f4 acc = (f4)0.f;
+#pragma unroll
+                    for (int f = 0; f < NF; f++) acc = dot(acc, fs[f], fa[it][f]);
+                    acc *= F16 ? carry[it] * (s_up * p_down) : carry[it];
+                    O[it][v] = dot(acc, fct[v], fp[it]);
+                }
+            }
+            // The weight zero times an infinity or NaN of a later token is NaN: such a chunk is done again token by token.
+            if (n_tok > 1) {
+                float z = 0.f;
+#pragma unroll
+                for (int it = 0; it < NB; it++)
+#pragma unroll
+                    for (int v = 0; v < VB; v++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) z += O[it][v][r] * 0.f;
+                if (__any(z != z)) return false;
+            }
+            then();
+#pragma unroll
+            for (int it = 0; it < NB; it++)
+                if (16 * it + c < n_tok) {
+                    T* to = po + (int64_t)(x + 16 * it) * sto;
+                    constexpr int RUN = HALF ? 8 : 4 * VB;  // neighbouring columns
+#pragma unroll
+                    for (int q = 0; q < 4 * VB / RUN; q++) {
+                        int left = db - j0 - RUN * g - 32 * q;
+                        constexpr int N = MODE == EXACT ? 16 / sizeof(T) : MODE == FOURS ? 4 : 1;
+                        typedef T V __attribute__((ext_vector_type(N)));
+#pragma unroll
+                        for (int e = 0; e < RUN; e += N) {
+                            V y;
+#pragma unroll
+                            for (int i = 0; i < N; i++) {
+                                int v = HALF ? 2 * q + (e + i) / 4 : (e + i) % VB, r = HALF ? (e + i) % 4 : (e + i) / VB;
+                                y[i] = (T)(F16 ? O[it][v][r] * p_up : O[it][v][r]);
+                            }
+                            if (MODE == EXACT || e < left) *(V*)(to + 32 * q + e) = y;
+                        }
                     }
                 }
-
-        }  // !STATE
+        } else {
+            then();
+        }
 
         // the state: c weighted by its decay to the chunk's end.  In 16 bits the weighted value goes in as two parts of T, which
         // keeps the state as exact as float32 sums of this length are.  fp16 is brought to 2^14 .. 2^15 for it, where the second
@@ -409,29 +495,73 @@ __global__ __launch_bounds__(256) void k_sweep(Sweeps all) {
             unit(wave_max(most), &c_down, &c_up);
             c_down *= 16384.f, c_up *= 1.f / 16384.f, keep *= c_down;
         }
+        float by[FE];
+#pragma unroll
+        for (int e = 0; e < FE; e++) {
+            by[e] = enter[e];
+            if (n_tok < CH) {
+                int to = n_tok - (e / 4 * 16 + e % 4 + 4 * g) - w.e0;
+                by[e] = w.sb * power(lg, to > 0 ? to : 0);
+            }
+            if (F16) by[e] *= c_down;
+        }
+        u4 wbt[VA];
+        columns<L, RA, true, VA>(wbt, buf + L::B0, c, g);
+        if (n_tok < CH)
+#pragma unroll
+            for (int u = 0; u < VA; u++) wbt[u] &= tokens;
 #pragma unroll
         for (int v = 0; v < VB; v++) {
             Frag hi, lo;
 #pragma unroll
             for (int e = 0; e < FE; e++) {
-                float by = enter[e];
-                if (n_tok < CH) {
-                    int to = n_tok - (e / 4 * 16 + e % 4 + 4 * g) - w.e0;
-                    by = w.sb * power(lg, to > 0 ? to : 0);
-                }
-                float y = (float)fct[v][e] * (F16 ? by * c_down : by);
+                float y = (float)fct[v][e] * by[e];
                 hi[e] = (T)y;
                 if (HALF) lo[e] = (T)(y - (float)hi[e]);
             }
 #pragma unroll
             for (int u = 0; u < VA; u++) {
-                S[u][v] = dot(S[u][v] * keep, fbt[u], hi);
-                if (HALF) S[u][v] = dot(S[u][v], fbt[u], lo);
+                Frag b = __builtin_bit_cast(Frag, wbt[u]);
+                S[u][v] = dot(S[u][v] * keep, b, hi);
+                if (HALF) S[u][v] = dot(S[u][v], b, lo);
                 if (F16) S[u][v] *= c_up;
             }
         }
-        x += n_tok;
-        pa += n_tok * sta, pb += n_tok * stb, pbt += n_tok * stb, pct += n_tok * stc, po += n_tok * sto;
+        return true;
+    };
+
+    int x = 0;
+    bool fresh;
+    int n_tok = chunk(0, &fresh);
+    issue(0, 0, n_tok);
+    commit(0);
+    // one chunk, out of one half, while the next one's rows come into the other
+    auto turn = [&](auto half) {
+        constexpr int other = 1 - decltype(half)::value;
+        int x_next = x + n_tok, n_next = 0;
+        bool f_next = false;
+        if (x_next < steps) {
+            n_next = chunk(x_next, &f_next);
+            issue(other, x_next, n_next);
+        }
+        if (!compute(half, x, n_tok, fresh, [&] { commit(other); })) {
+            slow = x_next, n_tok = 1;
+            commit(other);  // the loads under way are for later tokens
+            issue(other, x, 1);
+            commit(other);
+            return;
+        }
+        x = x_next, n_tok = n_next, fresh = f_next;
+        if (flags && x - seen >= 64) {
+            m0 = m1, m1 = __ballot(ahead != 0), seen += 64;
+            ahead = flag(seen + 128 + lane);
+        }
+    };
+    while (true) {
+        turn(Int<0>());
+        if (x >= steps) break;
+        turn(Int<1>());
+        if (x >= steps) break;
     }
 
     if (STATE) {
@@ -450,8 +580,8 @@ __global__ __launch_bounds__(256) void k_sweep(Sweeps all) {
         for (int v = 0; v < VB; v++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                int i = VA * (4 * g + r) + u;
-                if (i < da && col + v < db) w.s_out[(int64_t)nh * da * db + i * w.s_i + (col + v) * w.s_j] = drop ? 0.f : w.out_mul * S[u][v][r];
+                int i = L::dim(u, 4 * g + r), j = j0 + L::col(v, c);
+                if (i < da && j < db) w.s_out[(int64_t)nh * da * db + i * w.s_i + j * w.s_j] = drop ? 0.f : w.out_mul * S[u][v][r];
             }
 }
 
@@ -460,9 +590,9 @@ __global__ __launch_bounds__(256) void k_sweep(Sweeps all) {
 // threads take a run of up to 16 segments each, all of whose loads are in flight at once, then hand on through LDS.
 constexpr int RUNS = 8, RUN = 16, MAX_SEGS = RUNS * RUN;
 
-template <int DA>
+template <class L>
 __global__ __launch_bounds__(256) void k_join(Sweeps all) {
-    constexpr int VA = DA / 16, VB = 2, TILES = VA * VB;
+    constexpr int VA = L::VA, VB = L::VB, TILES = VA * VB;
     __shared__ f4 sums[RUNS][32];
     __shared__ float lefts[RUNS];
     unsigned part = blockIdx.x % (2 * TILES), rest = blockIdx.x / (2 * TILES);
@@ -490,7 +620,7 @@ __global__ __launch_bounds__(256) void k_join(Sweeps all) {
     __syncthreads();
     int g = lane / 16, c = lane % 16, u = tile / VB, v = tile % VB;
 #pragma unroll
-    for (int r = 0; r < 4; r++) x[r] = entering(w, nh, VA * (4 * g + r) + u, slice * 16 * VB + VB * c + v);
+    for (int r = 0; r < 4; r++) x[r] = entering(w, nh, L::dim(u, 4 * g + r), slice * 16 * VB + L::col(v, c));
     for (int i = 0; i < run; i++) x = step(x, lefts[i], sums[i][threadIdx.x % 32]);
 #pragma unroll
     for (unsigned i = 0; i < RUN; i++)
@@ -500,37 +630,40 @@ __global__ __launch_bounds__(256) void k_join(Sweeps all) {
         }
 }
 
+// columns of C that a wave holds, by the tile width of a and b: wide tiles share their rows among more
+static constexpr int columns_of(int tile) { return tile <= 64 ? 32 : 64; }
+
 // every access of the tensor falls on multiples of `elements` elements
 static bool aligned(const Rows& r, int size, int elements) {
     return (uintptr_t)r.p % (size * elements) == 0 && r.st % elements == 0 && r.sn % elements == 0 && r.sh % elements == 0;
 }
 
-template <typename T, int DA>
-static void launch(const Sweeps& s, hipStream_t st) {
+template <typename T, class L>
+static void launch_tile(const Sweeps& s, hipStream_t st) {
     int mode = EXACT, unit = 16 / sizeof(T);
-    for (int i = 0; i < s.count; i++) {
+    for (unsigned i = 0; i < s.count; i++) {
         const Sweep& w = s.w[i];
         auto all = [&](int n) { return aligned(w.a, sizeof(T), n) && aligned(w.b, sizeof(T), n) && aligned(w.c, sizeof(T), n) && aligned(w.o, sizeof(T), n); };
-        if (mode == EXACT && !(w.da == DA && w.db % 32 == 0 && all(unit))) mode = FOURS;
+        if (mode == EXACT && !(w.da == L::DA && w.db % (16 * L::VB) == 0 && all(unit))) mode = FOURS;
         if (mode == FOURS && !(w.da % 4 == 0 && w.db % 4 == 0 && all(4))) mode = ANY;
     }
-    unsigned grid = (s.items + 3) / 4;
+    unsigned grid = (s.items + 7) / 8 * 8;
     if (s.segs > 1) {
-        if (mode == EXACT) k_sweep<T, DA, EXACT, true><<<grid, 256, 0, st>>>(s);
-        else if (mode == FOURS) k_sweep<T, DA, FOURS, true><<<grid, 256, 0, st>>>(s);
-        else k_sweep<T, DA, ANY, true><<<grid, 256, 0, st>>>(s);
-        k_join<DA><<<s.items / s.segs * (DA / 16 * 2) * 2, 256, 0, st>>>(s);
+        if (mode == EXACT) k_sweep<T, L, EXACT, true><<<grid, 64, 0, st>>>(s);
+        else if (mode == FOURS) k_sweep<T, L, FOURS, true><<<grid, 64, 0, st>>>(s);
+        else k_sweep<T, L, ANY, true><<<grid, 64, 0, st>>>(s);
+        k_join<L><<<s.items / s.segs * L::VA * L::VB * 2, 256, 0, st>>>(s);
     }
-    if (mode == EXACT) k_sweep<T, DA, EXACT, false><<<grid, 256, 0, st>>>(s);
-    else if (mode == FOURS) k_sweep<T, DA, FOURS, false><<<grid, 256, 0, st>>>(s);
-    else k_sweep<T, DA, ANY, false><<<grid, 256, 0, st>>>(s);
+    if (mode == EXACT) k_sweep<T, L, EXACT, false><<<grid, 64, 0, st>>>(s);
+    else if (mode == FOURS) k_sweep<T, L, FOURS, false><<<grid, 64, 0, st>>>(s);
+    else k_sweep<T, L, ANY, false><<<grid, 64, 0, st>>>(s);
 }
 
 template <typename T>
 static void launch(const Sweeps& s, hipStream_t st) {
-    if (s.w[0].da <= 32) launch<T, 32>(s, st);
-    else if (s.w[0].da <= 64) launch<T, 64>(s, st);
-    else launch<T, 128>(s, st);
+    if (s.w[0].da <= 32) launch_tile<T, Tile<T, 32, columns_of(32) / 16>>(s, st);
+    else if (s.w[0].da <= 64) launch_tile<T, Tile<T, 64, columns_of(64) / 16>>(s, st);
+    else launch_tile<T, Tile<T, 128, columns_of(128) / 16>>(s, st);
 }
 
 static int tile(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
@@ -542,7 +675,7 @@ static Sweeps plan(const urgym_ops_seq* q, const Sweep* w, int count) {
     s.count = count, s.heads = q->heads, s.steps = q->steps, s.log_decay = q->log_decay;
     for (int i = 0; i < count; i++) {
         s.w[i] = w[i];
-        unsigned n = (w[i].db + 31) / 32;
+        unsigned cols = columns_of(tile(w[i].da)), n = (w[i].db + cols - 1) / cols;
         s.slices = n > s.slices ? n : s.slices;
     }
     s.items = (unsigned)(q->envs * q->heads) * s.count * s.slices;
@@ -557,10 +690,10 @@ static Sweeps plan(const urgym_ops_seq* q, const Sweep* w, int count) {
     return s;
 }
 
-static int64_t workspace(const Sweeps& s) { return s.segs > 1 ? (int64_t)s.items * (tile(s.w[0].da) * 32 + 1) : 0; }
+static int64_t workspace(const Sweeps& s) { return s.segs > 1 ? (int64_t)s.items * (tile(s.w[0].da) * columns_of(tile(s.w[0].da)) + 1) : 0; }
 
 static void launch(const urgym_ops_seq* q, Sweeps s, float* ws, hipStream_t st) {
-    s.ws = ws, s.left = ws + (int64_t)s.items * tile(s.w[0].da) * 32;
+    s.ws = ws, s.left = ws + (int64_t)s.items * tile(s.w[0].da) * columns_of(tile(s.w[0].da));
     if (q->dtype == URGYM_OPS_F32) launch<float>(s, st);
     else if (q->dtype == URGYM_OPS_BF16) launch<bf16>(s, st);
     else launch<f16>(s, st);
