@@ -12,7 +12,8 @@
 //   o_i = sa g^(i + e0) C^T a_i + sum_{j <= i} sa sb g^(i - j) (a_i . b_j) c_j
 //   C  <- g^n C + sum_j sb g^(n - j - e0) b_j c_j^T         (e0 = 1 forward, 0 backward)
 // which are matrix products.  A chunk ends where the next episode begins, so every chunk lies in one episode and the only mask
-// is i >= j; rows past its end are zeroed by selection, so that nothing of another episode, a NaN included, is ever multiplied.
+// is i >= j.  A shorter chunk's n tokens are the last of the CH rows, which leaves all weights but those of the carried state as
+// they are; the rows before them are zeroed, so that nothing of another episode, a NaN included, is ever multiplied.
 //
 // One wave (a workgroup of its own: no barrier) holds 16 VB columns of one (env, head)'s C in the accumulators of 16x16 matrix
 // instructions for the whole sweep.  While a chunk is computed with, the next one's rows are on their way from memory into the
@@ -146,13 +147,6 @@ __device__ __forceinline__ void load_to_lds(unsigned to, const void* from) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
 }
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
-// N words, or zeros where the mask is zero (a selection: nothing of what is dropped is computed with)
-template <int N>
-__device__ __forceinline__ void only(unsigned* x, unsigned mask) {
-#pragma unroll
-    for (int i = 0; i < N; i++) x[i] &= mask;
-}
 
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
@@ -311,7 +305,7 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
     };
 
     // A chunk's rows into one half of LDS: `issue`, then (loads that pass through registers) `commit`, then `landed`.  Lane by lane
-    // 16 bytes; rows past the chunk's end are its last one's, zeroed before they are used.
+    // 16 bytes; the rows before a short chunk's are its first one's, zeroed before they are used.
     constexpr int KA = CH * RA / 1024, KC = CH * RC / 1024;
     unsigned stage[MODE == EXACT ? 1 : 2 * KA + KC][4];
     const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
@@ -321,7 +315,7 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
         for (int k = 0; k < K; k++) {
             int t = k * (1024 / RB) + lane / (RB / 16);
             int byte = place<RB>(t, lane * 16 % RB) - t * RB;  // exchanging units twice is nothing: what belongs at this place
-            int64_t tt = n_tok == CH || t < n_tok ? t : n_tok - 1;
+            int64_t tt = n_tok == CH ? t : t < CH - n_tok ? 0 : t - (CH - n_tok);
             const T* from = base + tt * st + byte / (int)sizeof(T);
             if constexpr (MODE == EXACT) load_to_lds(__builtin_amdgcn_readfirstlane(at + buf * L::BUF + tile0 + k * 1024), from);
             else fetch<T, MODE>(stage[k0 + k], from, byte / (int)sizeof(T), width);
@@ -344,7 +338,7 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
     // One chunk from LDS: o, then the state; `then` runs in between, before o is stored.  False (and nothing done) where the chunk
     // has to be taken token by token.
     auto compute = [&](auto half, int x, int n_tok, bool fresh, auto then) {
-        const char* buf = lds + decltype(half)::value * L::BUF;
+        char* buf = lds + decltype(half)::value * L::BUF;
         if (fresh) {
             any = 1;
 #pragma unroll
@@ -352,22 +346,18 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
 #pragma unroll
                 for (int v = 0; v < VB; v++) S[u][v] = (f4)0.f;
         }
+        if (n_tok < CH) {
+            auto zero = [&](auto size, int tile0) {
+                constexpr int RB = decltype(size)::value;
+#pragma unroll
+                for (int k = 0; k < CH * RB / 1024; k++)
+                    if (k * (1024 / RB) + lane / (RB / 16) < CH - n_tok) *(u4*)(buf + tile0 + k * 1024 + lane * 16) = (u4)0u;
+            };
+            if (!STATE) zero(Int<RA>(), L::A0);
+            zero(Int<RA>(), L::B0), zero(Int<RC>(), L::C0);
+        }
         u4 wct[VB];
         columns<L, RC, false, VB>(wct, buf + L::C0, c, g);
-        u4 tokens = (u4)~0u;  // which of an operand's tokens exist
-        if (n_tok < CH) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (HALF) {
-                    int t = 16 * (i / 2) + 4 * g + 2 * (i % 2);
-                    tokens[i] = (t < n_tok ? 0xffffu : 0u) | (t + 1 < n_tok ? 0xffff0000u : 0u);
-                } else {
-                    tokens[i] = 4 * g + i < n_tok ? ~0u : 0u;
-                }
-            }
-#pragma unroll
-            for (int v = 0; v < VB; v++) wct[v] &= tokens;
-        }
         Frag fct[VB];
 #pragma unroll
         for (int v = 0; v < VB; v++) fct[v] = __builtin_bit_cast(Frag, wct[v]);
@@ -380,16 +370,13 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int f = 0; f < NF; f++) {
-                    u4 wa = row<L, RA>(buf + L::A0, 16 * b + c, f, g);
-                    if (n_tok < CH) wa &= 16 * b + c < n_tok ? ~0u : 0u;
-                    fa[b][f] = __builtin_bit_cast(Frag, wa);
+                    fa[b][f] = __builtin_bit_cast(Frag, row<L, RA>(buf + L::A0, 16 * b + c, f, g));
                 }
 #pragma unroll
             for (int jb = 0; jb < NB; jb++)
 #pragma unroll
                 for (int f = 0; f < NF; f++) {
                     u4 wb = row<L, RA>(buf + L::B0, 16 * jb + c, f, g);
-                    if (n_tok < CH) wb &= 16 * jb + c < n_tok ? ~0u : 0u;
 #pragma unroll
                     for (int it = jb; it < NB; it++) sc[it][jb] = dot(f ? sc[it][jb] : (f4)0.f, __builtin_bit_cast(Frag, wb), fa[it][f]);
                 }
@@ -422,6 +409,15 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
             // here: an error of half a step of T in each product, as large as that of the output's own rounding.
             f4 O[NB][VB];
             Frag fp[NB];
+            float by_token[NB];
+#pragma unroll
+            for (int it = 0; it < NB; it++) by_token[it] = carry[it];
+            if (n_tok < CH)
+#pragma unroll
+                for (int it = 0; it < NB; it++) {
+                    int i = 16 * it + c - (CH - n_tok);
+                    by_token[it] = w.sa * power(lg, (i > 0 ? i : 0) + w.e0);
+                }
 #pragma unroll
             for (int it = 0; it < NB; it++)
 #pragma unroll
@@ -439,7 +435,7 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
                     f4 acc = (f4)0.f;
 #pragma unroll
                     for (int f = 0; f < NF; f++) acc = dot(acc, fs[f], fa[it][f]);
-                    acc *= F16 ? carry[it] * (s_up * p_down) : carry[it];
+                    acc *= F16 ? by_token[it] * (s_up * p_down) : by_token[it];
                     O[it][v] = dot(acc, fct[v], fp[it]);
                 }
             }
@@ -457,8 +453,8 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
             then();
 #pragma unroll
             for (int it = 0; it < NB; it++)
-                if (16 * it + c < n_tok) {
-                    T* to = po + (int64_t)(x + 16 * it) * sto;
+                if (16 * it + c >= CH - n_tok) {
+                    T* to = po + (int64_t)(x + 16 * it - (CH - n_tok)) * sto;
                     constexpr int RUN = HALF ? 8 : 4 * VB;  // neighbouring columns
 #pragma unroll
                     for (int q = 0; q < 4 * VB / RUN; q++) {
@@ -495,27 +491,14 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
             unit(wave_max(most), &c_down, &c_up);
             c_down *= 16384.f, c_up *= 1.f / 16384.f, keep *= c_down;
         }
-        float by[FE];
-#pragma unroll
-        for (int e = 0; e < FE; e++) {
-            by[e] = enter[e];
-            if (n_tok < CH) {
-                int to = n_tok - (e / 4 * 16 + e % 4 + 4 * g) - w.e0;
-                by[e] = w.sb * power(lg, to > 0 ? to : 0);
-            }
-            if (F16) by[e] *= c_down;
-        }
         u4 wbt[VA];
         columns<L, RA, true, VA>(wbt, buf + L::B0, c, g);
-        if (n_tok < CH)
-#pragma unroll
-            for (int u = 0; u < VA; u++) wbt[u] &= tokens;
 #pragma unroll
         for (int v = 0; v < VB; v++) {
             Frag hi, lo;
 #pragma unroll
             for (int e = 0; e < FE; e++) {
-                float y = (float)fct[v][e] * by[e];
+                float y = (float)fct[v][e] * (F16 ? enter[e] * c_down : enter[e]);
                 hi[e] = (T)y;
                 if (HALF) lo[e] = (T)(y - (float)hi[e]);
             }
