@@ -16,13 +16,14 @@
 // they are; the rows before them are zeroed, so that nothing of another episode, a NaN included, is ever multiplied.
 //
 // One wave (a workgroup of its own: no barrier) holds 16 VB columns of one (env, head)'s C in the accumulators of 16x16 matrix
-// instructions for the whole sweep.  While a chunk is computed with, the next one's rows are on their way from memory into the
-// other half of the wave's LDS, without passing through registers.  The operands' layouts meet (c = lane % 16, g = lane / 16):
+// instructions for the whole sweep.  A chunk's operands are read out of LDS at once; while they are computed with, the next chunk's
+// rows are on their way from memory into the same LDS, without passing through registers.  The operands' layouts meet
+// (c = lane % 16, g = lane / 16):
 //   * an accumulator holds rows 4 g + r of column c; as the next product's operand its lane holds 4 elements of the contracted
 //     axis at 4 g + r.  Scores (b a^T, transposed) feed the product with c, and C the product with a, after a conversion only;
 //   * o is computed transposed, so that a lane holds neighbouring columns of one token, which it stores as a vector;
 //   * 16-bit operands that contract the tokens are transposed on their way out of LDS.
-// LDS rows are swizzled in units of 32 bytes, so that both kinds of reads spread over the banks.
+// LDS rows are swizzled in blocks of 16 bytes, so that both kinds of reads spread over the banks.
 #include "uo_common.h"
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -82,23 +83,25 @@ struct FragOf<f16> {
     typedef f16x8 type;
 };
 
-// A wave's tiles: CH tokens of a and b (DA wide) and of 16 VB columns of c, in LDS twice
+// A wave's tiles in LDS: CH tokens of a and b (DA wide) and of 16 VB columns of c
 template <typename T, int DA_, int VB_>
 struct Tile {
     static constexpr int DA = DA_, VB = VB_, ES = sizeof(T), FE = 16 / ES, NB = FE / 4, CH = 16 * NB, NF = DA / 4 / FE, VA = DA / 16;
     static constexpr int RA = DA * ES, RC = 16 * VB * ES;  // bytes of a row
     static constexpr int A0 = 0, B0 = CH * RA, C0 = 2 * CH * RA, BUF = 2 * CH * RA + CH * RC;
-    // the dimension of row m of C's tile u, and the column (of the wave's) of its column m of tile v
-    static __device__ __forceinline__ int dim(int u, int m) { return ES == 2 ? 16 * u + m : VA * m + u; }
+    // the dimension of row m of C's tile u, and the column (of the wave's) of its column m of tile v: in 16 bits 4 + 4 elements of
+    // two tiles are 16 neighbouring bytes, in 32 the tiles' elements alternate
+    static __device__ __forceinline__ int dim(int u, int m) { return ES == 2 ? 32 * (u / 2) + 8 * (m / 4) + 4 * (u % 2) + m % 4 : VA * m + u; }
     static __device__ __forceinline__ int col(int v, int m) { return ES == 2 ? 32 * (v / 2) + 8 * (m / 4) + 4 * (v % 2) + m % 4 : VB * m + v; }
 };
 
-// where byte `byte` of row t lies in a tile of RB bytes a row: 32-byte units, exchanged so that 8 neighbouring units of one column
-// of units (8 rows at least) fall on 256 different bytes
+// where byte `byte` of row t lies in a tile of RB bytes a row: blocks of 16 bytes are exchanged so that 8 rows' blocks of one column
+// of blocks fall on 8 different places of 128 bytes (reads of rows), and 4 rows' four blocks on two of each (transposed reads)
 template <int RB>
 __device__ __forceinline__ int place(int t, int byte) {
-    constexpr int U = RB / 32, R = U >= 8 ? 1 : 8 / U;
-    return t * RB + ((byte / 32 ^ t / R % U) * 32) + byte % 32;
+    constexpr int N = RB / 16;
+    int s = N >= 8 ? (t & 1) << 2 | (t >> 1 & 3) : t / 2 % 4;
+    return t * RB + ((byte / 16 ^ s) * 16) + byte % 16;
 }
 
 // acc += a b over the fragments' contracted axis (32 deep in 16 bits, 4 x 4 in 32)
@@ -112,8 +115,8 @@ __device__ __forceinline__ f4 dot(f4 acc, f4 a, f4 b) {
 
 __device__ __forceinline__ float power(float lg, int n) { return n == 0 ? 1.f : exp2f(lg * (float)n); }
 
-// How rows are fetched.  EXACT: widths are the tiles' and everything is 16-byte aligned: from memory into LDS directly.  Otherwise
-// through registers, 4 elements at a time where widths and offsets are multiples of 4 (FOURS), or one (ANY).
+// How rows are fetched.  EXACT: widths are the tiles', everything is 16-byte aligned and a chunk lies within 2 GiB: from memory into
+// LDS directly.  Otherwise through registers, 4 elements at a time where widths and offsets are multiples of 4 (FOURS), or one (ANY).
 enum { EXACT, FOURS, ANY };
 
 // 16 bytes of elements at p as words; of those from column col on, the ones below width exist
@@ -140,11 +143,10 @@ __device__ __forceinline__ void fetch(unsigned* to, const T* p, int col, int wid
     }
 }
 
-// 16 bytes of each lane's address to LDS bytes to .. to + 1023, lane by lane.  Written as assembly because the compiler would wait
-// for it before the next read of LDS, whichever half that reads; the waits are `landed`.  (m0, the address in LDS, has no other
-// use in these kernels.)
-__device__ __forceinline__ void load_to_lds(unsigned to, const void* from) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+// 16 bytes at base + each lane's offset to LDS bytes to .. to + 1023, lane by lane.  Written as assembly because the compiler would
+// wait for it before the next read of LDS; the waits are `landed`.  (m0, the address in LDS, has no other use in these kernels.)
+__device__ __forceinline__ void load_to_lds(unsigned to, const void* base, unsigned offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
 }
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -152,26 +154,20 @@ typedef unsigned u4 __attribute__((ext_vector_type(4)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
 
 // Fragments from LDS, as words.  `row`: row t of a tile, the f-th part of it (operand with the dimensions contracted);
-// `column`: tile u of its columns with the tokens contracted (DIM: a's and b's dimensions, else c's columns).
+// `columns`: N tiles of its columns with the tokens contracted.
 template <class L, int RB>
 __device__ __forceinline__ u4 row(const char* tile, int t, int f, int g) {
-    if constexpr (L::ES == 2) {
-        u2 lo = *(const u2*)(tile + place<RB>(t, 64 * f + 8 * g)), hi = *(const u2*)(tile + place<RB>(t, 64 * f + 32 + 8 * g));
-        return u4{lo[0], lo[1], hi[0], hi[1]};
-    } else {
-        return *(const u4*)(tile + place<RB>(t, g * (RB / 4) + 16 * f));
-    }
+    return *(const u4*)(tile + place<RB>(t, L::ES == 2 ? 64 * f + 16 * g : g * (RB / 4) + 16 * f));
 }
 
-template <class L, int RB, bool DIM, int N>
+template <class L, int RB, int N>
 __device__ __forceinline__ void columns(u4* to, const char* tile, int c, int g) {
     if constexpr (L::ES == 2) {
         typedef short s4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s4* P;
 #pragma unroll
         for (int u = 0; u < N; u++) {
-            int byte = DIM ? 32 * u + 8 * (c % 4) : 64 * (u / 2) + 16 * (c % 4) + 8 * (u % 2);
-            const char* at = tile + place<RB>(4 * g + c / 4, byte);
+            const char* at = tile + place<RB>(4 * g + c / 4, 64 * (u / 2) + 16 * (c % 4) + 8 * (u % 2));
             u2 lo = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at)));
             u2 hi = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at + 16 * RB)));
             to[u] = u4{lo[0], lo[1], hi[0], hi[1]};
@@ -216,12 +212,14 @@ __device__ __forceinline__ f4* held(const Sweeps& all, unsigned item, int tiles,
 }
 
 // STATE: only what the segment adds to the state (no a, no o); segments after it need that before they can begin.
+// Two waves a SIMD at least, that is 256 registers at most: then matrix instructions accumulate in ordinary registers, where C is
+// scaled and converted between any two of them.
 template <typename T, class L, int MODE, bool STATE>
-__global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
+__global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
     typedef typename FragOf<T>::type Frag;
     constexpr int FE = L::FE, NB = L::NB, CH = L::CH, NF = L::NF, VA = L::VA, VB = L::VB, RA = L::RA, RC = L::RC;
     constexpr bool HALF = Kind<T>::HALF, F16 = Kind<T>::F16;
-    __shared__ __attribute__((aligned(256))) char lds[2 * L::BUF];
+    __shared__ __attribute__((aligned(256))) char lds[L::BUF];
     // workgroups go to the 8 XCDs in turn: each takes a run of items, for neighbours share rows -- the slices, then the sweeps,
     // then the heads of one env -- and their L2
     unsigned item = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
@@ -243,7 +241,9 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
     // o: token c, the lane's run of 4 VB columns (float32) or its runs of 8 (16 bits: one in every 32)
     T* const po = (T*)w.o.p + n * w.o.sn + h * w.o.sh + (x0 + c) * sto + j0 + (HALF ? 8 : 4 * VB) * g;
 
+    // C = unit * S: a chunk's decay goes into the unit, and into the tokens that enter, instead of into all of S
     f4 S[VA][VB];
+    float s_unit = 1.f;
 #pragma unroll
     for (int u = 0; u < VA; u++)
 #pragma unroll
@@ -304,48 +304,46 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
         return x < slow ? 1 : n_tok;
     };
 
-    // A chunk's rows into one half of LDS: `issue`, then (loads that pass through registers) `commit`, then `landed`.  Lane by lane
-    // 16 bytes; the rows before a short chunk's are its first one's, zeroed before they are used.
+    // A chunk's rows into LDS: `issue`, then `commit`, which waits (or writes what passes through registers).  Lane by lane 16 bytes; the rows before a short chunk's are its first one's, zeroed before they are used.
     constexpr int KA = CH * RA / 1024, KC = CH * RC / 1024;
     unsigned stage[MODE == EXACT ? 1 : 2 * KA + KC][4];
     const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-    auto rows_of = [&](auto size, auto part, int k0, const T* base, int64_t st, int tile0, int width, int n_tok, int buf) {
-        constexpr int RB = decltype(size)::value, K = decltype(part)::value;
+    auto rows_of = [&](auto size, auto part, int k0, const T* base, int64_t st, int tile0, int width, int x, int n_tok) {
+        constexpr int RB = decltype(size)::value, K = decltype(part)::value, ROWS = 1024 / RB;  // rows of one load
+        const int l = lane / (RB / 16);
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            int t = k * (1024 / RB) + lane / (RB / 16);
-            int byte = place<RB>(t, lane * 16 % RB) - t * RB;  // exchanging units twice is nothing: what belongs at this place
-            int64_t tt = n_tok == CH ? t : t < CH - n_tok ? 0 : t - (CH - n_tok);
-            const T* from = base + tt * st + byte / (int)sizeof(T);
-            if constexpr (MODE == EXACT) load_to_lds(__builtin_amdgcn_readfirstlane(at + buf * L::BUF + tile0 + k * 1024), from);
-            else fetch<T, MODE>(stage[k0 + k], from, byte / (int)sizeof(T), width);
+            int t = k * ROWS + l, ts = ROWS % 8 ? t : l;
+            int byte = place<RB>(ts, lane * 16 % RB) - ts * RB;  // exchanging blocks twice is nothing: what belongs at this place
+            int tt = n_tok == CH ? t : t < CH - n_tok ? 0 : t - (CH - n_tok);
+            if constexpr (MODE == EXACT) {  // offsets are unsigned: from the load's lowest row, the last one of a backward sweep
+                unsigned size = (unsigned)(st < 0 ? -st : st) * sizeof(T);
+                int low = n_tok == CH ? k * ROWS : 0, row = n_tok == CH ? l : tt, last = n_tok == CH ? ROWS - 1 : n_tok - 1;
+                const T* from = base + (int64_t)(x + low + (st < 0 ? last : 0)) * st;
+                load_to_lds(at + tile0 + k * 1024, from, (unsigned)(st < 0 ? last - row : row) * size + byte);
+            } else {
+                fetch<T, MODE>(stage[k0 + k], base + (int64_t)(x + tt) * st + byte / (int)sizeof(T), byte / (int)sizeof(T), width);
+            }
         }
     };
-    auto issue = [&](int buf, int x, int n_tok) {
-        if (MODE == EXACT) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every read of this half has been answered
-        if (!STATE) rows_of(Int<RA>(), Int<KA>(), 0, pa + x * sta, sta, L::A0, da, n_tok, buf);
-        rows_of(Int<RA>(), Int<KA>(), KA, pb + x * stb, stb, L::B0, da, n_tok, buf);
-        rows_of(Int<RC>(), Int<KC>(), 2 * KA, pc + x * stc, stc, L::C0, db - j0, n_tok, buf);
+    auto issue = [&](int x, int n_tok) {
+        if (MODE == EXACT) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every read has been answered
+        if (!STATE) rows_of(Int<RA>(), Int<KA>(), 0, pa, sta, L::A0, da, x, n_tok);
+        rows_of(Int<RA>(), Int<KA>(), KA, pb, stb, L::B0, da, x, n_tok);
+        rows_of(Int<RC>(), Int<KC>(), 2 * KA, pc, stc, L::C0, db - j0, x, n_tok);
     };
-    auto commit = [&](int buf) {
+    auto commit = [&] {
         if constexpr (MODE == EXACT) landed();
         else
 #pragma unroll
             for (int k = STATE ? KA : 0; k < 2 * KA + KC; k++)
-                *(u4*)(lds + buf * L::BUF + k * 1024 + lane * 16) = u4{stage[k][0], stage[k][1], stage[k][2], stage[k][3]};
+                *(u4*)(lds + k * 1024 + lane * 16) = u4{stage[k][0], stage[k][1], stage[k][2], stage[k][3]};
     };
 
-    // One chunk from LDS: o, then the state; `then` runs in between, before o is stored.  False (and nothing done) where the chunk
-    // has to be taken token by token.
-    auto compute = [&](auto half, int x, int n_tok, bool fresh, auto then) {
-        char* buf = lds + decltype(half)::value * L::BUF;
-        if (fresh) {
-            any = 1;
-#pragma unroll
-            for (int u = 0; u < VA; u++)
-#pragma unroll
-                for (int v = 0; v < VB; v++) S[u][v] = (f4)0.f;
-        }
+    // One chunk: the operands from LDS, then (`next`: the next chunk's loads begin) o and the state, then (`done`: they have landed)
+    // the stores.  False, and nothing done, where the chunk has to be taken token by token.
+    auto compute = [&](int x, int n_tok, bool fresh, auto next, auto done) {
+        char* buf = lds;
         if (n_tok < CH) {
             auto zero = [&](auto size, int tile0) {
                 constexpr int RB = decltype(size)::value;
@@ -357,37 +355,59 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
             zero(Int<RA>(), L::B0), zero(Int<RC>(), L::C0);
         }
         u4 wct[VB];
-        columns<L, RC, false, VB>(wct, buf + L::C0, c, g);
+        columns<L, RC, VB>(wct, buf + L::C0, c, g);
         Frag fct[VB];
 #pragma unroll
         for (int v = 0; v < VB; v++) fct[v] = __builtin_bit_cast(Frag, wct[v]);
-
-        if constexpr (!STATE) {
-            // scores, transposed: row j = 4 g + r, column i = c
-            Frag fa[NB][NF];
-            f4 sc[NB][NB];
+        // The score zero of a later token times its c is zero, or NaN where c is an infinity or NaN (as the product with a matrix of
+        // zeros tells): a chunk with such tokens is taken one by one.
+        if (!STATE && n_tok > 1) {
+            float z = 0.f;
+#pragma unroll
+            for (int v = 0; v < VB; v++) z += dot((f4)0.f, (Frag)(T)0.f, fct[v])[0];
+            if (__any(z != z)) return false;
+        }
+        Frag fa[STATE ? 1 : NB][NF], fb[STATE ? 1 : NB][NF], fbt[VA];
+        if constexpr (!STATE)
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int f = 0; f < NF; f++) {
                     fa[b][f] = __builtin_bit_cast(Frag, row<L, RA>(buf + L::A0, 16 * b + c, f, g));
+                    fb[b][f] = __builtin_bit_cast(Frag, row<L, RA>(buf + L::B0, 16 * b + c, f, g));
                 }
+        u4 wbt[VA];
+        columns<L, RA, VA>(wbt, buf + L::B0, c, g);
+#pragma unroll
+        for (int u = 0; u < VA; u++) fbt[u] = __builtin_bit_cast(Frag, wbt[u]);
+        next();
+        if (fresh) {
+            any = 1, s_unit = 1.f;
+#pragma unroll
+            for (int u = 0; u < VA; u++)
+#pragma unroll
+                for (int v = 0; v < VB; v++) S[u][v] = (f4)0.f;
+        }
+
+        f4 O[NB][VB];
+        float p_up = 1.f;
+        if constexpr (!STATE) {
+            // scores, transposed: row j = 4 g + r, column i = c
+            f4 sc[NB][NB];
 #pragma unroll
             for (int jb = 0; jb < NB; jb++)
 #pragma unroll
-                for (int f = 0; f < NF; f++) {
-                    u4 wb = row<L, RA>(buf + L::B0, 16 * jb + c, f, g);
+                for (int f = 0; f < NF; f++)
 #pragma unroll
-                    for (int it = jb; it < NB; it++) sc[it][jb] = dot(f ? sc[it][jb] : (f4)0.f, __builtin_bit_cast(Frag, wb), fa[it][f]);
-                }
+                    for (int it = jb; it < NB; it++) sc[it][jb] = dot(f ? sc[it][jb] : (f4)0.f, fb[jb][f], fa[it][f]);
             float p[NB][FE];
 #pragma unroll
             for (int it = 0; it < NB; it++)
 #pragma unroll
                 for (int jb = 0; jb < NB; jb++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) p[it][4 * jb + r] = jb < it ? sc[it][jb][r] * far[r] : jb == it ? sc[it][jb][r] * near[r] : 0.f;
-            float p_down = 1.f, p_up = 1.f, s_down = 1.f, s_up = 1.f;
+                    for (int r = 0; r < 4; r++) p[it][4 * jb + r] = jb < it ? sc[it][jb][r] * far[r] : jb == it && c >= 4 * g + r ? sc[it][jb][r] * near[r] : 0.f;
+            float p_down = 1.f, s_down = 1.f, s_up = 1.f;
             if constexpr (F16) {
                 float most = 0.f;
 #pragma unroll
@@ -407,16 +427,15 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
 
             // o, transposed: the carried state's part, weighted by token, then the chunk's own.  Scores and state are rounded to T
             // here: an error of half a step of T in each product, as large as that of the output's own rounding.
-            f4 O[NB][VB];
             Frag fp[NB];
             float by_token[NB];
 #pragma unroll
-            for (int it = 0; it < NB; it++) by_token[it] = carry[it];
+            for (int it = 0; it < NB; it++) by_token[it] = carry[it] * s_unit;
             if (n_tok < CH)
 #pragma unroll
                 for (int it = 0; it < NB; it++) {
                     int i = 16 * it + c - (CH - n_tok);
-                    by_token[it] = w.sa * power(lg, (i > 0 ? i : 0) + w.e0);
+                    by_token[it] = w.sa * power(lg, (i > 0 ? i : 0) + w.e0) * s_unit;
                 }
 #pragma unroll
             for (int it = 0; it < NB; it++)
@@ -439,18 +458,53 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
                     O[it][v] = dot(acc, fct[v], fp[it]);
                 }
             }
-            // The weight zero times an infinity or NaN of a later token is NaN: such a chunk is done again token by token.
-            if (n_tok > 1) {
-                float z = 0.f;
+        }
+
+        // the state: c weighted by its decay to the chunk's end.  In 16 bits the weighted value goes in as two parts of T, which
+        // keeps the state as exact as float32 sums of this length are.  S is touched only where the unit has become small, or, in
+        // fp16, where it does not bring this chunk's c into 2^6 .. 2^15, where both parts have their bits.
+        float keep = n_tok < CH ? power(lg, n_tok) : whole, unit_new = s_unit * keep;
+        bool off = unit_new < 1.f / 65536;
+        if constexpr (F16) {
+            float most = 0.f, down, up;
 #pragma unroll
-                for (int it = 0; it < NB; it++)
+            for (int v = 0; v < VB; v++)
 #pragma unroll
-                    for (int v = 0; v < VB; v++)
+                for (int e = 0; e < FE; e++) most = fmaxf(most, fabsf((float)fct[v][e]));
+            most = wave_max(most);
+            unit(most, &down, &up);
+            off = off || !(most < unit_new * 32768.f) || (most < unit_new * 64.f && most > 0.f);
+            unit_new = off ? up * (1.f / 4096) : unit_new;
+        } else {
+            unit_new = off ? 1.f : unit_new;
+        }
+        if (__builtin_amdgcn_readfirstlane(off)) {
+            keep *= s_unit * __builtin_amdgcn_rcpf(unit_new);
 #pragma unroll
-                        for (int r = 0; r < 4; r++) z += O[it][v][r] * 0.f;
-                if (__any(z != z)) return false;
+            for (int u = 0; u < VA; u++)
+#pragma unroll
+                for (int v = 0; v < VB; v++) S[u][v] *= keep;
+        }
+        s_unit = unit_new;
+        const float grow = __builtin_amdgcn_rcpf(unit_new);
+#pragma unroll
+        for (int v = 0; v < VB; v++) {
+            Frag hi, lo;
+#pragma unroll
+            for (int e = 0; e < FE; e++) {
+                float y = (float)fct[v][e] * (enter[e] * grow);
+                asm("" : "+v"(y));  // y is rounded here: its product fused into one of the conversions would give that another hi
+                hi[e] = (T)y;
+                if (HALF) lo[e] = (T)(y - (float)hi[e]);
             }
-            then();
+#pragma unroll
+            for (int u = 0; u < VA; u++) {
+                S[u][v] = dot(S[u][v], fbt[u], hi);
+                if (HALF) S[u][v] = dot(S[u][v], fbt[u], lo);
+            }
+        }
+        done();
+        if constexpr (!STATE) {
 #pragma unroll
             for (int it = 0; it < NB; it++)
                 if (16 * it + c >= CH - n_tok) {
@@ -473,85 +527,39 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
                         }
                     }
                 }
-        } else {
-            then();
-        }
-
-        // the state: c weighted by its decay to the chunk's end.  In 16 bits the weighted value goes in as two parts of T, which
-        // keeps the state as exact as float32 sums of this length are.  fp16 is brought to 2^14 .. 2^15 for it, where the second
-        // part has its bits still, and the accumulators with it.
-        float keep = whole, c_down = 1.f, c_up = 1.f;
-        if (n_tok < CH) keep = power(lg, n_tok);
-        if constexpr (F16) {
-            float most = 0.f;
-#pragma unroll
-            for (int v = 0; v < VB; v++)
-#pragma unroll
-                for (int e = 0; e < FE; e++) most = fmaxf(most, fabsf((float)fct[v][e]));
-            unit(wave_max(most), &c_down, &c_up);
-            c_down *= 16384.f, c_up *= 1.f / 16384.f, keep *= c_down;
-        }
-        u4 wbt[VA];
-        columns<L, RA, true, VA>(wbt, buf + L::B0, c, g);
-#pragma unroll
-        for (int v = 0; v < VB; v++) {
-            Frag hi, lo;
-#pragma unroll
-            for (int e = 0; e < FE; e++) {
-                float y = (float)fct[v][e] * (F16 ? enter[e] * c_down : enter[e]);
-                hi[e] = (T)y;
-                if (HALF) lo[e] = (T)(y - (float)hi[e]);
-            }
-#pragma unroll
-            for (int u = 0; u < VA; u++) {
-                Frag b = __builtin_bit_cast(Frag, wbt[u]);
-                S[u][v] = dot(S[u][v] * keep, b, hi);
-                if (HALF) S[u][v] = dot(S[u][v], b, lo);
-                if (F16) S[u][v] *= c_up;
-            }
         }
         return true;
     };
 
-    int x = 0;
     bool fresh;
     int n_tok = chunk(0, &fresh);
-    issue(0, 0, n_tok);
-    commit(0);
-    // one chunk, out of one half, while the next one's rows come into the other
-    auto turn = [&](auto half) {
-        constexpr int other = 1 - decltype(half)::value;
-        int x_next = x + n_tok, n_next = 0;
+    issue(0, n_tok);
+    commit();
+    for (int x = 0; x < steps;) {
+        const int x_next = x + n_tok;
         bool f_next = false;
-        if (x_next < steps) {
-            n_next = chunk(x_next, &f_next);
-            issue(other, x_next, n_next);
-        }
-        if (!compute(half, x, n_tok, fresh, [&] { commit(other); })) {
+        const int n_next = x_next < steps ? chunk(x_next, &f_next) : 0;
+        auto begin = [&] {
+            if (n_next) issue(x_next, n_next);
+        };
+        if (!compute(x, n_tok, fresh, begin, commit)) {
             slow = x_next, n_tok = 1;
-            commit(other);  // the loads under way are for later tokens
-            issue(other, x, 1);
-            commit(other);
-            return;
+            issue(x, 1);
+            commit();
+            continue;
         }
         x = x_next, n_tok = n_next, fresh = f_next;
         if (flags && x - seen >= 64) {
             m0 = m1, m1 = __ballot(ahead != 0), seen += 64;
             ahead = flag(seen + 128 + lane);
         }
-    };
-    while (true) {
-        turn(Int<0>());
-        if (x >= steps) break;
-        turn(Int<1>());
-        if (x >= steps) break;
     }
 
     if (STATE) {
 #pragma unroll
         for (int u = 0; u < VA; u++)
 #pragma unroll
-            for (int v = 0; v < VB; v++) *held(all, item, VA * VB, u * VB + v, lane) = S[u][v];
+            for (int v = 0; v < VB; v++) *held(all, item, VA * VB, u * VB + v, lane) = S[u][v] * s_unit;
         if (lane == 0) all.left[item] = any ? 0.f : power(lg, steps);
         return;
     }
@@ -564,7 +572,7 @@ __global__ __launch_bounds__(64) void k_sweep(Sweeps all) {
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 int i = L::dim(u, 4 * g + r), j = j0 + L::col(v, c);
-                if (i < da && j < db) w.s_out[(int64_t)nh * da * db + i * w.s_i + j * w.s_j] = drop ? 0.f : w.out_mul * S[u][v][r];
+                if (i < da && j < db) w.s_out[(int64_t)nh * da * db + i * w.s_i + j * w.s_j] = drop ? 0.f : w.out_mul * s_unit * S[u][v][r];
             }
 }
 
@@ -613,8 +621,9 @@ __global__ __launch_bounds__(256) void k_join(Sweeps all) {
         }
 }
 
-// columns of C that a wave holds, by the tile width of a and b: wide tiles share their rows among more
-static constexpr int columns_of(int tile) { return tile <= 64 ? 32 : 64; }
+// Columns of C that a wave holds, by the tile width of a and b: as many as its registers take, for they share the scores.  (32 wide
+// tiles would take 64 too, but then leave half of a wave's columns empty for heads of 32.)
+static constexpr int columns_of(int tile) { return tile == 64 ? 64 : 32; }
 
 // every access of the tensor falls on multiples of `elements` elements
 static bool aligned(const Rows& r, int size, int elements) {
@@ -627,7 +636,9 @@ static void launch_tile(const Sweeps& s, hipStream_t st) {
     for (unsigned i = 0; i < s.count; i++) {
         const Sweep& w = s.w[i];
         auto all = [&](int n) { return aligned(w.a, sizeof(T), n) && aligned(w.b, sizeof(T), n) && aligned(w.c, sizeof(T), n) && aligned(w.o, sizeof(T), n); };
-        if (mode == EXACT && !(w.da == L::DA && w.db % (16 * L::VB) == 0 && all(unit))) mode = FOURS;
+        auto near = [](const Rows& r) { return (r.st < 0 ? -r.st : r.st) < ((int64_t)1 << 31) / ((int)sizeof(T) * L::CH); };  // 32-bit offsets
+        bool exact = w.da == L::DA && w.db % (16 * L::VB) == 0 && all(unit) && near(w.a) && near(w.b) && near(w.c);
+        if (mode == EXACT && !exact) mode = FOURS;
         if (mode == FOURS && !(w.da % 4 == 0 && w.db % 4 == 0 && all(4))) mode = ANY;
     }
     unsigned grid = (s.items + 7) / 8 * 8;
