@@ -283,7 +283,9 @@ def test_step_strides(ops):
     moved = torch.zeros(state.numel() + 1, device=DEV)[1:].view(state.shape)  # a state off 16-byte alignment
     moved.copy_(state)
     got = ops.decay_attention_step(q[0], k[0], v[0], g, moved, start[0], state_out=moved)
-    assert torch.equal(got[0], want[0]) and torch.equal(moved, want[1])
+    assert torch.equal(moved, want[1])  # each element is one product and one sum, in any layout
+    refs, bounds = decay_bounds((q, k, v, g, state, start), {}, torch.bfloat16)
+    assert_close(got[0], refs[0][0], bounds[0][0])  # o's sum runs in another order there: each order is within its bound
 
 
 # ---- layer norm ----

@@ -57,6 +57,7 @@ struct Sweep {
 struct Sweeps {
     Sweep w[3];
     unsigned count, slices, segs, heads;  // sweeps in this launch, waves for each of them and segment of the axis, segments
+    int columns;                          // of C that a wave holds
     unsigned items;                       // envs * heads * count * slices * segs waves
     int seg_len;                          // steps in a segment (the last may be shorter)
     int64_t steps;
@@ -578,10 +579,10 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
 
 // The states that the segments begin with, from what each adds: begin_0 = what enters, begin_{s+1} = left_s begin_s + added_s
 // (selected where left_s = 0, so that nothing passes a start).  A workgroup takes 32 float4s of one wave's accumulators; its 8 rows of
-// threads take a run of up to 16 segments each, all of whose loads are in flight at once, then hand on through LDS.
-constexpr int RUNS = 8, RUN = 16, MAX_SEGS = RUNS * RUN;
+// threads take a run of PER segments each, all of whose loads are in flight at once, then hand on through LDS.
+constexpr int RUNS = 8, MAX_SEGS = RUNS * 16;
 
-template <class L>
+template <class L, int PER>
 __global__ __launch_bounds__(256) void k_join(Sweeps all) {
     constexpr int VA = L::VA, VB = L::VB, TILES = VA * VB;
     __shared__ f4 sums[RUNS][32];
@@ -590,40 +591,41 @@ __global__ __launch_bounds__(256) void k_join(Sweeps all) {
     unsigned slice = rest % all.slices, role = rest / all.slices % all.count, nh = rest / all.slices / all.count;
     const Sweep& w = all.w[role];
     if ((int)slice * 16 * VB >= w.db) return;
-    int tile = part / 2, lane = part % 2 * 32 + threadIdx.x % 32, run = threadIdx.x / 32;
-    unsigned per = (all.segs + RUNS - 1) / RUNS, s0 = run * per;
+    const int tile = part / 2, lane = part % 2 * 32 + threadIdx.x % 32, run = threadIdx.x / 32;
+    const unsigned s0 = run * PER;
     auto item = [&](unsigned s) { return ((nh * all.segs + s) * all.count + role) * all.slices + slice; };
     auto step = [](f4 x, float left, f4 add) { return left == 0.f ? add : x * left + add; };
-    f4 add[RUN];
-    float left[RUN];
+    f4 add[PER], begin;
+    float left[PER];
+    int g = lane / 16, c = lane % 16, u = tile / VB, v = tile % VB;
 #pragma unroll
-    for (unsigned i = 0; i < RUN; i++) {
-        bool in = i < per && s0 + i < all.segs;
+    for (int r = 0; r < 4; r++) begin[r] = entering(w, nh, L::dim(u, 4 * g + r), slice * 16 * VB + L::col(v, c));
+#pragma unroll
+    for (unsigned i = 0; i < PER; i++) {
+        bool in = s0 + i < all.segs;
         add[i] = in ? *held(all, item(s0 + i), TILES, tile, lane) : (f4)0.f;
         left[i] = in ? all.left[item(s0 + i)] : 1.f;
     }
     f4 x = (f4)0.f;
     float l = 1.f;
 #pragma unroll
-    for (int i = 0; i < RUN; i++) x = step(x, left[i], add[i]), l *= left[i];
+    for (int i = 0; i < PER; i++) x = step(x, left[i], add[i]), l *= left[i];
     sums[run][threadIdx.x % 32] = x;
     if (threadIdx.x % 32 == 0) lefts[run] = l;
     __syncthreads();
-    int g = lane / 16, c = lane % 16, u = tile / VB, v = tile % VB;
-#pragma unroll
-    for (int r = 0; r < 4; r++) x[r] = entering(w, nh, L::dim(u, 4 * g + r), slice * 16 * VB + L::col(v, c));
+    x = begin;
     for (int i = 0; i < run; i++) x = step(x, lefts[i], sums[i][threadIdx.x % 32]);
 #pragma unroll
-    for (unsigned i = 0; i < RUN; i++)
-        if (i < per && s0 + i < all.segs) {
+    for (unsigned i = 0; i < PER; i++)
+        if (s0 + i < all.segs) {
             *held(all, item(s0 + i), TILES, tile, lane) = x;
             x = step(x, left[i], add[i]);
         }
 }
 
-// Columns of C that a wave holds, by the tile width of a and b: as many as its registers take, for they share the scores.  (32 wide
-// tiles would take 64 too, but then leave half of a wave's columns empty for heads of 32.)
-static constexpr int columns_of(int tile) { return tile == 64 ? 64 : 32; }
+// Columns of C that a wave holds, by the tile width of a and b and the width of c: as many as its registers take, for they share the
+// scores; 64 with tiles of 64 (500 x 1024 x 4 heads of 64: forward and backward 755 us, 865 with 32), where c has them.
+static int columns_of(int tile, int db) { return tile == 64 && db > 32 ? 64 : 32; }
 
 // every access of the tensor falls on multiples of `elements` elements
 static bool aligned(const Rows& r, int size, int elements) {
@@ -646,7 +648,10 @@ static void launch_tile(const Sweeps& s, hipStream_t st) {
         if (mode == EXACT) k_sweep<T, L, EXACT, true><<<grid, 64, 0, st>>>(s);
         else if (mode == FOURS) k_sweep<T, L, FOURS, true><<<grid, 64, 0, st>>>(s);
         else k_sweep<T, L, ANY, true><<<grid, 64, 0, st>>>(s);
-        k_join<L><<<s.items / s.segs * L::VA * L::VB * 2, 256, 0, st>>>(s);
+        unsigned parts = s.items / s.segs * L::VA * L::VB * 2;
+        if (s.segs <= RUNS) k_join<L, 1><<<parts, 256, 0, st>>>(s);
+        else if (s.segs <= 4 * RUNS) k_join<L, 4><<<parts, 256, 0, st>>>(s);
+        else k_join<L, 16><<<parts, 256, 0, st>>>(s);
     }
     if (mode == EXACT) k_sweep<T, L, EXACT, false><<<grid, 64, 0, st>>>(s);
     else if (mode == FOURS) k_sweep<T, L, FOURS, false><<<grid, 64, 0, st>>>(s);
@@ -655,9 +660,10 @@ static void launch_tile(const Sweeps& s, hipStream_t st) {
 
 template <typename T>
 static void launch(const Sweeps& s, hipStream_t st) {
-    if (s.w[0].da <= 32) launch_tile<T, Tile<T, 32, columns_of(32) / 16>>(s, st);
-    else if (s.w[0].da <= 64) launch_tile<T, Tile<T, 64, columns_of(64) / 16>>(s, st);
-    else launch_tile<T, Tile<T, 128, columns_of(128) / 16>>(s, st);
+    if (s.w[0].da <= 32) launch_tile<T, Tile<T, 32, 2>>(s, st);
+    else if (s.w[0].da <= 64 && s.columns == 64) launch_tile<T, Tile<T, 64, 4>>(s, st);
+    else if (s.w[0].da <= 64) launch_tile<T, Tile<T, 64, 2>>(s, st);
+    else launch_tile<T, Tile<T, 128, 2>>(s, st);
 }
 
 static int tile(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
@@ -667,11 +673,9 @@ static int tile(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 static Sweeps plan(const urgym_ops_seq* q, const Sweep* w, int count) {
     Sweeps s = {};
     s.count = count, s.heads = q->heads, s.steps = q->steps, s.log_decay = q->log_decay;
-    for (int i = 0; i < count; i++) {
-        s.w[i] = w[i];
-        unsigned cols = columns_of(tile(w[i].da)), n = (w[i].db + cols - 1) / cols;
-        s.slices = n > s.slices ? n : s.slices;
-    }
+    int db = 0;
+    for (int i = 0; i < count; i++) s.w[i] = w[i], db = w[i].db > db ? w[i].db : db;
+    s.columns = columns_of(tile(w[0].da), db), s.slices = (db + s.columns - 1) / s.columns;
     s.items = (unsigned)(q->envs * q->heads) * s.count * s.slices;
     int64_t segs = s.items >= 1024 ? 1 : 2048 / s.items, most = q->steps / 64;
     segs = segs < most ? segs : most;
@@ -684,35 +688,112 @@ static Sweeps plan(const urgym_ops_seq* q, const Sweep* w, int count) {
     return s;
 }
 
-static int64_t workspace(const Sweeps& s) { return s.segs > 1 ? (int64_t)s.items * (tile(s.w[0].da) * columns_of(tile(s.w[0].da)) + 1) : 0; }
+static int64_t workspace(const Sweeps& s) { return s.segs > 1 ? (int64_t)s.items * (tile(s.w[0].da) * s.columns + 1) : 0; }
 
 static void launch(const urgym_ops_seq* q, Sweeps s, float* ws, hipStream_t st) {
-    s.ws = ws, s.left = ws + (int64_t)s.items * tile(s.w[0].da) * columns_of(tile(s.w[0].da));
+    s.ws = ws, s.left = ws + (int64_t)s.items * tile(s.w[0].da) * s.columns;
     if (q->dtype == URGYM_OPS_F32) launch<float>(s, st);
     else if (q->dtype == URGYM_OPS_BF16) launch<bf16>(s, st);
     else launch<f16>(s, st);
 }
 
-// One wave per (env, head): lanes over the columns, the rows in turn.
-template <typename T>
-__global__ __launch_bounds__(64) void k_step(int heads, int dk, int dv, Rows q, Rows k, Rows v, const float* log_decay,
-                                             const uint8_t* start, int64_t start_sn, float scale, const float* s_in,
-                                             float* s_out, T* o) {
-    int64_t n = blockIdx.x / heads;
-    int h = blockIdx.x % heads;
-    float g = expf(log_decay[h]);
-    bool fresh = start && start[n * start_sn];
+// One token: W waves of a workgroup take one (env, head).  LPR lanes hold a row of the state, E elements each (neighbours, as one
+// vector, or LPR apart where dv is odd), and 64 / LPR rows are under way at once in each wave, 8 times over: the state's bytes, in and
+// out, are the whole cost.  The columns' sums over the rows are joined across lanes, then through LDS across the waves.
+template <typename T, int E, bool VEC, int LPR>
+__global__ __launch_bounds__(256) void k_step(int heads, int dk, int dv, Rows q, Rows k, Rows v, const float* log_decay,
+                                              const uint8_t* start, int64_t start_sn, float scale, const float* s_in,
+                                              float* s_out, T* o) {
+    constexpr int RPP = UO_WAVE / LPR, U = 8;
+    typedef float V __attribute__((ext_vector_type(VEC ? E : 1)));
+    __shared__ float qs[URGYM_OPS_MAX_HEAD_DIM], ks[URGYM_OPS_MAX_HEAD_DIM], sums[4][E * LPR];
+    const int64_t n = blockIdx.x / (unsigned)heads;
+    const int h = blockIdx.x % (unsigned)heads, waves = blockDim.x / UO_WAVE, wave = threadIdx.x / UO_WAVE, lane = threadIdx.x % UO_WAVE;
+    const int c = lane % LPR, r0 = wave * RPP + lane / LPR;
+    const bool fresh = start && start[n * start_sn];
     const T *qr = (const T*)q.p + n * q.sn + h * q.sh, *kr = (const T*)k.p + n * k.sn + h * k.sh, *vr = (const T*)v.p + n * v.sn + h * v.sh;
-    for (int j = threadIdx.x; j < dv; j += UO_WAVE) {
-        float x = (float)vr[j], acc = 0.f;
-        for (int i = 0; i < dk; i++) {
-            int64_t at = ((int64_t)blockIdx.x * dk + i) * dv + j;
-            float s = (fresh ? 0.f : g * s_in[at]) + (float)kr[i] * x;
-            s_out[at] = s;
-            acc += s * (float)qr[i];
+    auto col = [&](int e) { return VEC ? c * E + e : c + e * LPR; };
+    const float* in = s_in + (int64_t)blockIdx.x * dk * dv;
+    float* out = s_out + (int64_t)blockIdx.x * dk * dv;
+    float s[U][E], x[E], acc[E];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            int i = i0 + u * waves * RPP;
+#pragma unroll
+            for (int e = 0; e < E; e++) s[u][e] = 0.f;
+            if (i < dk && !fresh) {
+                if (VEC) {
+                    if (c * E < dv) {
+                        V y = *(const V*)(in + i * dv + c * E);
+#pragma unroll
+                        for (int e = 0; e < E; e++) s[u][e] = y[VEC ? e : 0];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        if (col(e) < dv) s[u][e] = in[i * dv + col(e)];
+                }
+            }
         }
-        o[(int64_t)blockIdx.x * dv + j] = (T)(scale * acc);
+    };
+    load(r0);
+    const float g = power(log_decay[h] * 1.44269504088896340736f, 1);
+    for (int i = threadIdx.x; i < dk; i += blockDim.x) qs[i] = scale * (float)qr[i], ks[i] = (float)kr[i];
+#pragma unroll
+    for (int e = 0; e < E; e++) x[e] = col(e) < dv ? (float)vr[col(e)] : 0.f, acc[e] = 0.f;
+    __syncthreads();
+    for (int i0 = r0; i0 - r0 < dk; i0 += U * waves * RPP) {
+        if (i0 != r0) load(i0);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            int i = i0 + u * waves * RPP;
+            if (i < dk) {
+                float b = ks[i], a = qs[i];
+                V y;
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    s[u][e] = (fresh ? 0.f : g * s[u][e]) + b * x[e];
+                    acc[e] += s[u][e] * a;
+                    if (VEC) y[VEC ? e : 0] = s[u][e];
+                    else if (col(e) < dv) out[i * dv + col(e)] = s[u][e];
+                }
+                if (VEC && c * E < dv) *(V*)(out + i * dv + c * E) = y;
+            }
+        }
     }
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+#pragma unroll
+        for (int m = LPR; m < UO_WAVE; m *= 2) acc[e] += __shfl_xor(acc[e], m);
+        if (waves > 1 && lane < LPR) sums[wave][e * LPR + c] = acc[e];
+    }
+    if (waves > 1) {
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            for (int i = 1; i < waves; i++) acc[e] += sums[i][e * LPR + c];
+    }
+    if (lane < LPR)
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (col(e) < dv) o[(int64_t)blockIdx.x * dv + col(e)] = (T)acc[e];
+}
+
+template <typename T>
+static void step(int64_t envs, int heads, int dk, int dv, Rows q, Rows k, Rows v, const float* log_decay, const uint8_t* start,
+                 int64_t start_sn, float scale, const float* s_in, float* s_out, T* o, hipStream_t st) {
+    unsigned grid = (unsigned)(envs * heads);
+    bool vec = dv % 4 == 0 && (uintptr_t)s_in % 16 == 0 && (uintptr_t)s_out % 16 == 0;
+    int lanes = vec ? dv / 4 : dv, lpr = lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
+    int rounds = (dk * lpr + UO_WAVE - 1) / UO_WAVE;  // loads of one wave, 8 of which it has under way
+    unsigned block = rounds <= 8 ? 64 : rounds <= 16 ? 128 : 256;
+#define STEP(E, VEC, LPR) k_step<T, E, VEC, LPR><<<grid, block, 0, st>>>(heads, dk, dv, q, k, v, log_decay, start, start_sn, scale, s_in, s_out, o)
+    if (vec) lpr == 8 ? STEP(4, true, 8) : lpr == 16 ? STEP(4, true, 16) : STEP(4, true, 32);
+    else if (dv > 64) STEP(2, false, 64);
+    else lpr <= 16 ? STEP(1, false, 16) : lpr == 32 ? STEP(1, false, 32) : STEP(1, false, 64);
+#undef STEP
 }
 
 static int seq_check(const char* what, int dtype, int64_t steps, int64_t envs, int heads, int dk, int dv) {
@@ -825,10 +906,9 @@ extern "C" int urgym_ops_decay_step(int dtype, int64_t envs, int heads, int dk, 
     if (seq_check("urgym_ops_decay_step", dtype, 1, envs, heads, dk, dv)) return -1;
     if (!q || !k || !v || !log_decay || !state || !state_out || !o) return uo_fail("urgym_ops_decay_step: a pointer is missing");
     Rows rq = {q, 0, q_sn, q_sh}, rk = {k, 0, k_sn, k_sh}, rv = {v, 0, v_sn, v_sh};
-    unsigned grid = (unsigned)(envs * heads);
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == URGYM_OPS_F32) k_step<float><<<grid, 64, 0, st>>>(heads, dk, dv, rq, rk, rv, log_decay, start, start_stride, scale, state, state_out, (float*)o);
-    else if (dtype == URGYM_OPS_BF16) k_step<bf16><<<grid, 64, 0, st>>>(heads, dk, dv, rq, rk, rv, log_decay, start, start_stride, scale, state, state_out, (bf16*)o);
-    else k_step<f16><<<grid, 64, 0, st>>>(heads, dk, dv, rq, rk, rv, log_decay, start, start_stride, scale, state, state_out, (f16*)o);
+    if (dtype == URGYM_OPS_F32) step(envs, heads, dk, dv, rq, rk, rv, log_decay, start, start_stride, scale, state, state_out, (float*)o, st);
+    else if (dtype == URGYM_OPS_BF16) step(envs, heads, dk, dv, rq, rk, rv, log_decay, start, start_stride, scale, state, state_out, (bf16*)o, st);
+    else step(envs, heads, dk, dv, rq, rk, rv, log_decay, start, start_stride, scale, state, state_out, (f16*)o, st);
     return uo_launched("urgym_ops_decay_step");
 }
