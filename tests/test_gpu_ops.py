@@ -16,7 +16,6 @@ ALL = [torch.float32, torch.bfloat16, torch.float16]
 @pytest.fixture(scope="module")
 def ops(built):
     from urgym_amd import ops
-    ops.lib()
     return ops
 
 
@@ -218,6 +217,24 @@ def test_missing_gradients_and_scale(ops):
     o, final = ops.decay_attention(q, k, v, g, s, start, scale=0.3)
     (d,) = torch.autograd.grad((o, final), s, (do, dfinal))
     assert torch.equal(d, full[5])
+
+
+def test_gradients_of_gradients_are_refused(ops):
+    q, k, v, g, *_ = _case(3, 1, 1, 8, 8, torch.float32)
+    q.requires_grad_()
+    x = torch.randn(3, 8, device=DEV, requires_grad=True)
+    for y, leaf in ((ops.decay_attention(q, k, v, g)[0], q), (ops.layer_norm(x), x)):
+        with pytest.raises(RuntimeError, match="gradients of gradients"):
+            torch.autograd.grad(y.sum(), leaf, create_graph=True)
+
+
+def test_inputs_changed_before_the_backward_pass_are_noticed(ops):
+    q, k, v, g, *_ = _case(3, 1, 1, 8, 8, torch.float32)
+    q.requires_grad_()
+    o, _ = ops.decay_attention(q, k, v, g)
+    k.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
 
 
 def test_zero_lengths(ops):
@@ -424,10 +441,14 @@ def test_captured_rollout_step_and_training_step(ops):
 
 def test_nothing_is_written_beyond_the_outputs(ops):
     """the C entries on buffers inside larger ones: what lies before and behind stays as it was"""
-    L = ops.lib()
+    from urgym_amd.ops import _native
+    L = _native.lib()
+    codes = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
     for dtype in ALL:
         q, k, v, g, state, start, do, dfinal = _case(35, 3, 2, 24, 40, dtype, 0.1, True, seed=15)
-        s = ops._seq(q, k, v, g, state, start, 0.2)
+        s = _native.Seq(codes[dtype], 2, 24, 40, 35, 3, q.data_ptr(), k.data_ptr(), v.data_ptr())
+        s.q_stride[:], s.k_stride[:], s.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+        s.log_decay, s.start, s.start_stride[:], s.state, s.scale = g.data_ptr(), start.data_ptr(), start.stride(), state.data_ptr(), 0.2
 
         def framed(n, dt):
             return torch.full((n + 512,), 7.0, dtype=dt, device=DEV)
@@ -453,7 +474,7 @@ def test_nothing_is_written_beyond_the_outputs(ops):
         y, stats, dx, dw, db = framed(rows * width, dtype), framed(2 * rows, torch.float32), framed(rows * width, dtype), \
             framed(width, torch.float32), framed(width, torch.float32)
         ws = framed(L.urgym_ops_layer_norm_workspace(rows, width), torch.float32)
-        code, p = ops._DTYPES[dtype], lambda t, i=0: t[256 + i:].data_ptr()  # noqa: E731
+        code, p = codes[dtype], lambda t, i=0: t[256 + i:].data_ptr()  # noqa: E731
         assert L.urgym_ops_layer_norm(code, 0, rows, width, x.data_ptr(), width, w.data_ptr(), None, 1e-5, p(y), p(stats),
                                       p(stats, rows), stream) == 0
         assert L.urgym_ops_layer_norm_backward(code, 0, rows, width, x.data_ptr(), width, x.data_ptr(), width, w.data_ptr(),
