@@ -187,10 +187,14 @@ __device__ __forceinline__ void columns(u4* to, const char* tile, int c, int g) 
     }
 }
 
+// the largest of a wave's values, none of them negative
 __device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int m = 32; m; m >>= 1) x = fmaxf(x, __shfl_xor(x, m));
-    return x;
+    x = fmaxf(x, uo_dpp<0xB1>(x));   // lane ^ 1
+    x = fmaxf(x, uo_dpp<0x4E>(x));   // lane ^ 2
+    x = fmaxf(x, uo_dpp<0x141>(x));  // the mirror in 8
+    x = fmaxf(x, uo_dpp<0x140>(x));  // the mirror in 16
+    auto lane = [&](int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), i)); };
+    return fmaxf(fmaxf(lane(0), lane(16)), fmaxf(lane(32), lane(48)));
 }
 
 // 2^-e for a wave-wide largest magnitude in [2^e, 2^(e+1)), and 2^e; 1 for infinities and NaN.  fp16 operands are brought to about
@@ -202,9 +206,9 @@ __device__ __forceinline__ void unit(float most, float* down, float* up) {
     *down = __uint_as_float(0x7f000000u - e);
 }
 
-// element (i, j) of the state that enters the sweep
-__device__ __forceinline__ float entering(const Sweep& w, unsigned nh, int i, int j) {
-    return w.s_in && i < w.da && j < w.db ? w.in_mul * w.s_in[(int64_t)nh * w.da * w.db + i * w.s_i + j * w.s_j] : 0.f;
+// `by` times element (i, j) of the state that enters the sweep
+__device__ __forceinline__ float entering(const Sweep& w, unsigned nh, int i, int j, float by) {
+    return w.s_in && i < w.da && j < w.db ? by * w.s_in[(int64_t)nh * w.da * w.db + i * w.s_i + j * w.s_j] : 0.f;
 }
 
 // element (r, u, v) of a wave's accumulators in ws: float4s, lane by lane
@@ -242,9 +246,19 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
     // o: token c, the lane's run of 4 VB columns (float32) or its runs of 8 (16 bits: one in every 32)
     T* const po = (T*)w.o.p + n * w.o.sn + h * w.o.sh + (x0 + c) * sto + j0 + (HALF ? 8 : 4 * VB) * g;
 
+    // (Everything that has to come from memory is asked for first: the starts, the state, the first chunk.)
+    // the starts of tokens [seen, seen + 128) as two words; the third window's bytes are on their way
+    const uint8_t* flags = w.start ? w.start + n * w.start_sn + x0 * w.start_st : nullptr;
+    const bool first = w.first || seg;
+    auto flag = [&](int x) { return x < steps && (x || first) ? flags[x * w.start_st] : (uint8_t)0; };
+    uint64_t m0 = 0, m1 = 0, any = 0;
+    uint8_t f0 = 0, f1 = 0, ahead = 0;
+    int seen = 0;
+    if (flags) f0 = flag(lane), f1 = flag(64 + lane), ahead = flag(128 + lane);
+
     // C = unit * S: a chunk's decay goes into the unit, and into the tokens that enter, instead of into all of S
     f4 S[VA][VB];
-    float s_unit = 1.f;
+    float s_unit = STATE || all.segs > 1 || !w.s_in ? 1.f : w.in_mul;
 #pragma unroll
     for (int u = 0; u < VA; u++)
 #pragma unroll
@@ -255,38 +269,15 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
                 S[u][v] = *held(all, item, VA * VB, u * VB + v, lane);
             } else {
 #pragma unroll
-                for (int r = 0; r < 4; r++) S[u][v][r] = entering(w, nh, L::dim(u, 4 * g + r), j0 + L::col(v, c));
+                for (int r = 0; r < 4; r++) S[u][v][r] = entering(w, nh, L::dim(u, 4 * g + r), j0 + L::col(v, c), 1.f);
             }
         }
 
+    if (flags) m0 = __ballot(f0 != 0), m1 = __ballot(f1 != 0);
+
     // the scores' weights (i = c, j = 4 g + r; the other block of rows is 16 further), the rows' of the carried state, and the
     // tokens' on the state after a whole chunk
-    float near[4], far[4], carry[NB], enter[FE];
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-        int d = c - 4 * g - r;
-        near[r] = d >= 0 ? w.sa * w.sb * power(lg, d) : 0.f;
-        far[r] = w.sa * w.sb * power(lg, 16 + d);
-#pragma unroll
-        for (int b = 0; b < NB; b++) enter[4 * b + r] = w.sb * power(lg, CH - (16 * b + 4 * g + r) - w.e0);
-    }
-#pragma unroll
-    for (int b = 0; b < NB; b++) carry[b] = w.sa * power(lg, 16 * b + c + w.e0);
-    const float whole = power(lg, CH);
-
-    // the starts of tokens [seen, seen + 128) as two words; the third window's bytes are on their way
-    const uint8_t* flags = w.start ? w.start + n * w.start_sn + x0 * w.start_st : nullptr;
-    const bool first = w.first || seg;
-    auto flag = [&](int x) { return x < steps && (x || first) ? flags[x * w.start_st] : (uint8_t)0; };
-    uint64_t m0 = 0, m1 = 0, any = 0;
-    uint8_t ahead = 0;
-    int seen = 0;
-    if (flags) {
-        uint8_t f0 = flag(lane), f1 = flag(64 + lane);
-        ahead = flag(128 + lane);
-        m0 = __ballot(f0 != 0), m1 = __ballot(f1 != 0);
-    }
-
+    float near[4], far[4], carry[NB], enter[FE], whole;
     int slow = 0;  // tokens below it are taken one at a time
     // the chunk that begins at token x: its length, and whether an episode begins with it
     auto chunk = [&](int x, bool* fresh) {
@@ -535,6 +526,17 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
     bool fresh;
     int n_tok = chunk(0, &fresh);
     issue(0, n_tok);
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        int d = c - 4 * g - r;
+        near[r] = d >= 0 ? w.sa * w.sb * power(lg, d) : 0.f;
+        far[r] = w.sa * w.sb * power(lg, 16 + d);
+#pragma unroll
+        for (int b = 0; b < NB; b++) enter[4 * b + r] = w.sb * power(lg, CH - (16 * b + 4 * g + r) - w.e0);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; b++) carry[b] = w.sa * power(lg, 16 * b + c + w.e0);
+    whole = power(lg, CH);
     commit();
     for (int x = 0; x < steps;) {
         const int x_next = x + n_tok;
@@ -599,7 +601,7 @@ __global__ __launch_bounds__(256) void k_join(Sweeps all) {
     float left[PER];
     int g = lane / 16, c = lane % 16, u = tile / VB, v = tile % VB;
 #pragma unroll
-    for (int r = 0; r < 4; r++) begin[r] = entering(w, nh, L::dim(u, 4 * g + r), slice * 16 * VB + L::col(v, c));
+    for (int r = 0; r < 4; r++) begin[r] = entering(w, nh, L::dim(u, 4 * g + r), slice * 16 * VB + L::col(v, c), w.in_mul);
 #pragma unroll
     for (unsigned i = 0; i < PER; i++) {
         bool in = s0 + i < all.segs;
