@@ -11,9 +11,12 @@
 // The sweep runs in chunks of up to CH = 32 tokens (16 for float32).  With C the state before the chunk, i, j inside it:
 //   o_i = sa g^(i + e0) C^T a_i + sum_{j <= i} sa sb g^(i - j) (a_i . b_j) c_j
 //   C  <- g^n C + sum_j sb g^(n - j - e0) b_j c_j^T         (e0 = 1 forward, 0 backward)
-// which are matrix products.  A chunk ends where the next episode begins, so every chunk lies in one episode and the only mask
-// is i >= j.  A shorter chunk's n tokens are the last of the CH rows, which leaves all weights but those of the carried state as
-// they are; the rows before them are zeroed, so that nothing of another episode, a NaN included, is ever multiplied.
+// which are matrix products.  Where episodes begin inside a chunk, token i sees the tokens from its own episode's first on; the
+// carried state reaches the first episode's tokens and the last one's enter the new state, selected, not multiplied by zero.
+// The last chunk's n tokens are the last of the CH rows, which leaves all weights but those of the carried state as they
+// are; the rows before them are zeroed.  An infinity or NaN must not reach what does not see it, but times a weight of zero
+// it would: a chunk with one (in c; with several episodes, in b too) is cut where the next episode begins, and if that does not
+// help, into single tokens, which see nothing else.
 //
 // One wave (a workgroup of its own: no barrier) holds 16 VB columns of one (env, head)'s C in the accumulators of 16x16 matrix
 // instructions for the whole sweep.  A chunk's operands are read out of LDS at once; while they are computed with, the next chunk's
@@ -27,6 +30,8 @@
 #include "uo_common.h"
 
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -117,34 +122,47 @@ __device__ __forceinline__ f4 dot(f4 acc, f4 a, f4 b) {
     return acc;
 }
 
-__device__ __forceinline__ float power(float lg, int n) { return n == 0 ? 1.f : exp2f(lg * (float)n); }
+// 2^(lg n); 1 for n = 0, whatever lg
+__device__ __forceinline__ float power(float lg, int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(lg * (float)n); }
 
 // How rows are fetched.  EXACT: widths are the tiles', everything is 16-byte aligned and a chunk lies within 2 GiB: from memory into
 // LDS directly.  Otherwise through registers, 4 elements at a time where widths and offsets are multiples of 4 (FOURS), or one (ANY).
 enum { EXACT, FOURS, ANY };
 
-// 16 bytes of elements at p as words; of those from column col on, the ones below width exist
+// 16 bytes of elements as words, from column col of a row of `width` elements at p.  Columns that do not exist are read as the last
+// one (no branch holds up the loads after it); `present` zeroes them afterwards.
 template <typename T, int MODE>
 __device__ __forceinline__ void fetch(unsigned* to, const T* p, int col, int width) {
+    constexpr int N = 16 / sizeof(T);
     if constexpr (MODE == FOURS) {
         typedef unsigned V __attribute__((ext_vector_type(sizeof(T))));
 #pragma unroll
-        for (int i = 0; i < 4; i += sizeof(T)) {
-            V x = (V)0u;
-            if (col + i * 4 / (int)sizeof(T) < width) x = *(const V*)((const unsigned*)p + i);
+        for (int i = 0; i < N; i += 4) {
+            V x = *(const V*)(p + (col + i < width ? col + i : width - 4));
 #pragma unroll
-            for (int e = 0; e < (int)sizeof(T); e++) to[i + e] = x[e];
+            for (int e = 0; e < (int)sizeof(T); e++) to[i * (int)sizeof(T) / 4 + e] = x[e];
         }
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) to[i] = col + i < width ? ((const unsigned*)p)[i] : 0u;
+        for (int i = 0; i < N; i++) to[i] = ((const unsigned*)p)[col + i < width ? col + i : width - 1];
     } else {
+        unsigned x[N];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            unsigned lo = col + 2 * i < width ? ((const uint16_t*)p)[2 * i] : 0u;
-            to[i] = lo | (col + 2 * i + 1 < width ? (unsigned)((const uint16_t*)p)[2 * i + 1] << 16 : 0u);
-        }
+        for (int i = 0; i < N; i++) x[i] = ((const uint16_t*)p)[col + i < width ? col + i : width - 1];
+#pragma unroll
+        for (int i = 0; i < 4; i++) to[i] = x[2 * i] | x[2 * i + 1] << 16;
     }
+}
+
+template <typename T>
+__device__ __forceinline__ u4 present(const unsigned* from, int col, int width) {
+    u4 x;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) x[i] = col + i < width ? from[i] : 0u;
+        else x[i] = from[i] & ((col + 2 * i < width ? 0xffffu : 0u) | (col + 2 * i + 1 < width ? 0xffff0000u : 0u));
+    }
+    return x;
 }
 
 // 16 bytes at base + each lane's offset to LDS bytes to .. to + 1023, lane by lane.  Written as assembly because the compiler would
@@ -153,9 +171,6 @@ __device__ __forceinline__ void load_to_lds(unsigned to, const void* base, unsig
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
 }
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
-typedef unsigned u4 __attribute__((ext_vector_type(4)));
-typedef unsigned u2 __attribute__((ext_vector_type(2)));
 
 // Fragments from LDS, as words.  `row`: row t of a tile, the f-th part of it (operand with the dimensions contracted);
 // `columns`: N tiles of its columns with the tokens contracted.
@@ -281,22 +296,20 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
     // the scores' weights (i = c, j = 4 g + r; the other block of rows is 16 further), the rows' of the carried state, and the
     // tokens' on the state after a whole chunk
     float near[4], far[4], carry[NB], enter[FE], whole;
-    int slow = 0;  // tokens below it are taken one at a time
-    // the chunk that begins at token x: its length, and whether an episode begins with it
-    auto chunk = [&](int x, bool* fresh) {
-        int n_tok = steps - x < CH ? steps - x : CH;
-        *fresh = false;
+    int slow = 0, cut = 0;  // tokens below `slow` are taken one at a time, chunks below `cut` end with their episode
+    // the chunk that begins at token x: its length, whether an episode begins with it, and the tokens inside it that begin one
+    auto chunk = [&](int x, bool* fresh, unsigned* inside) {
+        int n_tok = x < slow ? 1 : steps - x < CH ? steps - x : CH;
+        *fresh = false, *inside = 0;
         if (flags) {
             int at = x - seen;
             uint64_t m = at == 0 ? m0 : at < 64 ? m0 >> at | m1 << (64 - at) : m1 >> (at - 64);
             *fresh = m & 1;
-            uint64_t next = m & ~1ull;
-            if (next) {
-                int d = __builtin_ctzll(next);
-                n_tok = d < n_tok ? d : n_tok;
-            }
+            unsigned next = (unsigned)m & (unsigned)((1ull << n_tok) - 2);
+            if (next && x < cut) n_tok = __builtin_ctz(next);
+            else *inside = next;
         }
-        return x < slow ? 1 : n_tok;
+        return n_tok;
     };
 
     // A chunk's rows into LDS: `issue`, then `commit`, which waits (or writes what passes through registers).  Lane by lane 16 bytes; the rows before a short chunk's are its first one's, zeroed before they are used.
@@ -317,7 +330,7 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
                 const T* from = base + (int64_t)(x + low + (st < 0 ? last : 0)) * st;
                 load_to_lds(at + tile0 + k * 1024, from, (unsigned)(st < 0 ? last - row : row) * size + byte);
             } else {
-                fetch<T, MODE>(stage[k0 + k], base + (int64_t)(x + tt) * st + byte / (int)sizeof(T), byte / (int)sizeof(T), width);
+                fetch<T, MODE>(stage[k0 + k], base + (int64_t)(x + tt) * st, byte / (int)sizeof(T), width);
             }
         }
     };
@@ -328,16 +341,26 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         rows_of(Int<RC>(), Int<KC>(), 2 * KA, pc, stc, L::C0, db - j0, x, n_tok);
     };
     auto commit = [&] {
-        if constexpr (MODE == EXACT) landed();
-        else
+        if constexpr (MODE == EXACT) {
+            landed();
+        } else {
+            auto put = [&](auto size, auto part, int k0, int tile0, int width) {
+                constexpr int RB = decltype(size)::value, K = decltype(part)::value, ROWS = 1024 / RB;
 #pragma unroll
-            for (int k = STATE ? KA : 0; k < 2 * KA + KC; k++)
-                *(u4*)(lds + k * 1024 + lane * 16) = u4{stage[k][0], stage[k][1], stage[k][2], stage[k][3]};
+                for (int k = 0; k < K; k++) {
+                    int l = lane / (RB / 16), ts = ROWS % 8 ? k * ROWS + l : l, byte = place<RB>(ts, lane * 16 % RB) - ts * RB;
+                    *(u4*)(lds + tile0 + k * 1024 + lane * 16) = present<T>(stage[k0 + k], byte / (int)sizeof(T), width);
+                }
+            };
+            if (!STATE) put(Int<RA>(), Int<KA>(), 0, L::A0, da);
+            put(Int<RA>(), Int<KA>(), KA, L::B0, da);
+            put(Int<RC>(), Int<KC>(), 2 * KA, L::C0, db - j0);
+        }
     };
 
     // One chunk: the operands from LDS, then (`next`: the next chunk's loads begin) o and the state, then (`done`: they have landed)
-    // the stores.  False, and nothing done, where the chunk has to be taken token by token.
-    auto compute = [&](int x, int n_tok, bool fresh, auto next, auto done) {
+    // the stores.  False, and nothing done, where the chunk has to be taken in parts.
+    auto compute = [&](int x, int n_tok, bool fresh, unsigned inside, auto next, auto done) {
         char* buf = lds;
         if (n_tok < CH) {
             auto zero = [&](auto size, int tile0) {
@@ -354,9 +377,8 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         Frag fct[VB];
 #pragma unroll
         for (int v = 0; v < VB; v++) fct[v] = __builtin_bit_cast(Frag, wct[v]);
-        // The score zero of a later token times its c is zero, or NaN where c is an infinity or NaN (as the product with a matrix of
-        // zeros tells): a chunk with such tokens is taken one by one.
-        if (!STATE && n_tok > 1) {
+        // (whether there is an infinity or NaN, the product with a matrix of zeros tells)
+        if (n_tok > 1 && (!STATE || inside)) {
             float z = 0.f;
 #pragma unroll
             for (int v = 0; v < VB; v++) z += dot((f4)0.f, (Frag)(T)0.f, fct[v])[0];
@@ -375,6 +397,23 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         columns<L, RA, VA>(wbt, buf + L::B0, c, g);
 #pragma unroll
         for (int u = 0; u < VA; u++) fbt[u] = __builtin_bit_cast(Frag, wbt[u]);
+        // the row from which on row i's episode lies in the chunk (0: from before it), and the last row's
+        int from[NB], last = 0;
+#pragma unroll
+        for (int b = 0; b < NB; b++) from[b] = 0;
+        if (inside) {
+            float z = 0.f;
+#pragma unroll
+            for (int u = 0; u < VA; u++) z += dot((f4)0.f, (Frag)(T)0.f, fbt[u])[0];
+            if (__any(z != z)) return false;
+            unsigned begins = inside << (CH - n_tok);
+            last = 31 - __builtin_clz(begins);
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                unsigned before = begins & (2u << (16 * b + c)) - 1;
+                from[b] = before ? 31 - __builtin_clz(before) : 0;
+            }
+        }
         next();
         if (fresh) {
             any = 1, s_unit = 1.f;
@@ -402,6 +441,11 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
                 for (int jb = 0; jb < NB; jb++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) p[it][4 * jb + r] = jb < it ? sc[it][jb][r] * far[r] : jb == it && c >= 4 * g + r ? sc[it][jb][r] * near[r] : 0.f;
+            if (inside)
+#pragma unroll
+                for (int it = 0; it < NB; it++)
+#pragma unroll
+                    for (int e = 0; e < FE; e++) p[it][e] = e / 4 * 16 + e % 4 + 4 * g >= from[it] ? p[it][e] : 0.f;
             float p_down = 1.f, s_down = 1.f, s_up = 1.f;
             if constexpr (F16) {
                 float most = 0.f;
@@ -450,6 +494,7 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
 #pragma unroll
                     for (int f = 0; f < NF; f++) acc = dot(acc, fs[f], fa[it][f]);
                     acc *= F16 ? by_token[it] * (s_up * p_down) : by_token[it];
+                    if (inside && from[it]) acc = (f4)0.f;
                     O[it][v] = dot(acc, fct[v], fp[it]);
                 }
             }
@@ -459,7 +504,7 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         // keeps the state as exact as float32 sums of this length are.  S is touched only where the unit has become small, or, in
         // fp16, where it does not bring this chunk's c into 2^6 .. 2^15, where both parts have their bits.
         float keep = n_tok < CH ? power(lg, n_tok) : whole, unit_new = s_unit * keep;
-        bool off = unit_new < 1.f / 65536;
+        bool off = unit_new < 1.f / 65536 || inside;
         if constexpr (F16) {
             float most = 0.f, down, up;
 #pragma unroll
@@ -478,16 +523,20 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
 #pragma unroll
             for (int u = 0; u < VA; u++)
 #pragma unroll
-                for (int v = 0; v < VB; v++) S[u][v] *= keep;
+                for (int v = 0; v < VB; v++) S[u][v] = inside ? (f4)0.f : S[u][v] * keep;
         }
+        if (inside) any = 1;
         s_unit = unit_new;
         const float grow = __builtin_amdgcn_rcpf(unit_new);
+        float by[FE];
+#pragma unroll
+        for (int e = 0; e < FE; e++) by[e] = !inside || e / 4 * 16 + e % 4 + 4 * g >= last ? enter[e] * grow : 0.f;
 #pragma unroll
         for (int v = 0; v < VB; v++) {
             Frag hi, lo;
 #pragma unroll
             for (int e = 0; e < FE; e++) {
-                float y = (float)fct[v][e] * (enter[e] * grow);
+                float y = (float)fct[v][e] * by[e];
                 asm("" : "+v"(y));  // y is rounded here: its product fused into one of the conversions would give that another hi
                 hi[e] = (T)y;
                 if (HALF) lo[e] = (T)(y - (float)hi[e]);
@@ -527,7 +576,8 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
     };
 
     bool fresh;
-    int n_tok = chunk(0, &fresh);
+    unsigned inside;
+    int n_tok = chunk(0, &fresh, &inside);
     issue(0, n_tok);
 #pragma unroll
     for (int r = 0; r < 4; r++) {
@@ -544,17 +594,19 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
     for (int x = 0; x < steps;) {
         const int x_next = x + n_tok;
         bool f_next = false;
-        const int n_next = x_next < steps ? chunk(x_next, &f_next) : 0;
+        unsigned i_next = 0;
+        const int n_next = x_next < steps ? chunk(x_next, &f_next, &i_next) : 0;
         auto begin = [&] {
             if (n_next) issue(x_next, n_next);
         };
-        if (!compute(x, n_tok, fresh, begin, commit)) {
-            slow = x_next, n_tok = 1;
-            issue(x, 1);
+        if (!compute(x, n_tok, fresh, inside, begin, commit)) {
+            (inside ? cut : slow) = x_next;
+            n_tok = chunk(x, &fresh, &inside);
+            issue(x, n_tok);
             commit();
             continue;
         }
-        x = x_next, n_tok = n_next, fresh = f_next;
+        x = x_next, n_tok = n_next, fresh = f_next, inside = i_next;
         if (flags && x - seen >= 64) {
             m0 = m1, m1 = __ballot(ahead != 0), seen += 64;
             ahead = flag(seen + 128 + lane);
