@@ -68,9 +68,12 @@ struct Sweeps {
     int64_t steps;
     const float* log_decay;
     // segs > 1: for each wave what its segment adds to the state, or (after k_join) the state it begins with, as the wave's
-    // accumulators lie in its registers; and the factor that it leaves of the state before it
+    // accumulators lie in its registers; and the factor that it leaves of the state before it.  Up to OWN_JOIN segments, each
+    // wave joins what lies before its own.
     float *ws, *left;
 };
+
+constexpr unsigned OWN_JOIN = 8;
 
 template <typename T>
 struct Kind {
@@ -234,6 +237,9 @@ __device__ __forceinline__ f4* held(const Sweeps& all, unsigned item, int tiles,
     return (f4*)all.ws + ((int64_t)item * tiles + tile) * UO_WAVE + lane;
 }
 
+// the state after a segment that leaves `left` of x and adds `add` (selected where it leaves nothing: nothing passes a start)
+__device__ __forceinline__ f4 joined(f4 x, float left, f4 add) { return left == 0.f ? add : x * left + add; }
+
 // STATE: only what the segment adds to the state (no a, no o); segments after it need that before they can begin.
 // Two waves a SIMD at least, that is 256 registers at most: then matrix instructions accumulate in ordinary registers, where C is
 // scaled and converted between any two of them.
@@ -276,20 +282,31 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
 
     // C = unit * S: a chunk's decay goes into the unit, and into the tokens that enter, instead of into all of S
     f4 S[VA][VB];
-    float s_unit = STATE || all.segs > 1 || !w.s_in ? 1.f : w.in_mul;
+    float s_unit = STATE || all.segs > OWN_JOIN || !w.s_in ? 1.f : w.in_mul;
 #pragma unroll
     for (int u = 0; u < VA; u++)
 #pragma unroll
         for (int v = 0; v < VB; v++) {
             if (STATE) {
                 S[u][v] = (f4)0.f;
-            } else if (all.segs > 1) {
+            } else if (all.segs > OWN_JOIN) {
                 S[u][v] = *held(all, item, VA * VB, u * VB + v, lane);
             } else {
 #pragma unroll
                 for (int r = 0; r < 4; r++) S[u][v][r] = entering(w, nh, L::dim(u, 4 * g + r), j0 + L::col(v, c), 1.f);
             }
         }
+    if (!STATE && all.segs <= OWN_JOIN) {
+        for (unsigned before = seg; before; before--) {
+            unsigned other = item - before * all.count * all.slices;
+            float left = all.left[other] * s_unit;
+#pragma unroll
+            for (int u = 0; u < VA; u++)
+#pragma unroll
+                for (int v = 0; v < VB; v++) S[u][v] = joined(S[u][v], left, *held(all, other, VA * VB, u * VB + v, lane));
+            s_unit = 1.f;
+        }
+    }
 
     if (flags) m0 = __ballot(f0 != 0), m1 = __ballot(f1 != 0);
 
@@ -634,8 +651,8 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
             }
 }
 
-// The states that the segments begin with, from what each adds: begin_0 = what enters, begin_{s+1} = left_s begin_s + added_s
-// (selected where left_s = 0, so that nothing passes a start).  A workgroup takes 32 float4s of one wave's accumulators; its 8 rows of
+// The states that the segments begin with, from what each adds: begin_0 = what enters, begin_{s+1} = left_s begin_s + added_s.
+// A workgroup takes 32 float4s of one wave's accumulators; its 8 rows of
 // threads take a run of PER segments each, all of whose loads are in flight at once, then hand on through LDS.
 constexpr int RUNS = 8, MAX_SEGS = RUNS * 16;
 
@@ -651,7 +668,6 @@ __global__ __launch_bounds__(256) void k_join(Sweeps all) {
     const int tile = part / 2, lane = part % 2 * 32 + threadIdx.x % 32, run = threadIdx.x / 32;
     const unsigned s0 = run * PER;
     auto item = [&](unsigned s) { return ((nh * all.segs + s) * all.count + role) * all.slices + slice; };
-    auto step = [](f4 x, float left, f4 add) { return left == 0.f ? add : x * left + add; };
     f4 add[PER], begin;
     float left[PER];
     int g = lane / 16, c = lane % 16, u = tile / VB, v = tile % VB;
@@ -666,23 +682,26 @@ __global__ __launch_bounds__(256) void k_join(Sweeps all) {
     f4 x = (f4)0.f;
     float l = 1.f;
 #pragma unroll
-    for (int i = 0; i < PER; i++) x = step(x, left[i], add[i]), l *= left[i];
+    for (int i = 0; i < PER; i++) x = joined(x, left[i], add[i]), l *= left[i];
     sums[run][threadIdx.x % 32] = x;
     if (threadIdx.x % 32 == 0) lefts[run] = l;
     __syncthreads();
     x = begin;
-    for (int i = 0; i < run; i++) x = step(x, lefts[i], sums[i][threadIdx.x % 32]);
+    for (int i = 0; i < run; i++) x = joined(x, lefts[i], sums[i][threadIdx.x % 32]);
 #pragma unroll
     for (unsigned i = 0; i < PER; i++)
         if (s0 + i < all.segs) {
             *held(all, item(s0 + i), TILES, tile, lane) = x;
-            x = step(x, left[i], add[i]);
+            x = joined(x, left[i], add[i]);
         }
 }
 
+constexpr int64_t FILL = 1024;  // waves: one for each SIMD
+
 // Columns of C that a wave holds, by the tile width of a and b and the width of c: as many as its registers take, for they share the
-// scores; 64 with tiles of 64 (500 x 1024 x 4 heads of 64: forward and backward 755 us, 865 with 32), where c has them.
-static int columns_of(int tile, int db) { return tile == 64 && db > 32 ? 64 : 32; }
+// scores; 64 with tiles of 64 (500 x 1024 x 4 heads of 64: forward and backward 755 us, 865 with 32), where c has them and the
+// waves fill the chip (with fewer, the time of one wave's chunk counts).
+static int columns_of(int tile, int db, int64_t waves) { return tile == 64 && db > 32 && waves >= FILL ? 64 : 32; }
 
 // every access of the tensor falls on multiples of `elements` elements
 static bool aligned(const Rows& r, int size, int elements) {
@@ -706,9 +725,8 @@ static void launch_tile(const Sweeps& s, hipStream_t st) {
         else if (mode == FOURS) k_sweep<T, L, FOURS, true><<<grid, 64, 0, st>>>(s);
         else k_sweep<T, L, ANY, true><<<grid, 64, 0, st>>>(s);
         unsigned parts = s.items / s.segs * L::VA * L::VB * 2;
-        if (s.segs <= RUNS) k_join<L, 1><<<parts, 256, 0, st>>>(s);
-        else if (s.segs <= 4 * RUNS) k_join<L, 4><<<parts, 256, 0, st>>>(s);
-        else k_join<L, 16><<<parts, 256, 0, st>>>(s);
+        if (s.segs > 4 * RUNS) k_join<L, 16><<<parts, 256, 0, st>>>(s);
+        else if (s.segs > OWN_JOIN) k_join<L, 4><<<parts, 256, 0, st>>>(s);
     }
     if (mode == EXACT) k_sweep<T, L, EXACT, false><<<grid, 64, 0, st>>>(s);
     else if (mode == FOURS) k_sweep<T, L, FOURS, false><<<grid, 64, 0, st>>>(s);
@@ -732,9 +750,9 @@ static Sweeps plan(const urgym_ops_seq* q, const Sweep* w, int count) {
     s.count = count, s.heads = q->heads, s.steps = q->steps, s.log_decay = q->log_decay;
     int db = 0;
     for (int i = 0; i < count; i++) s.w[i] = w[i], db = w[i].db > db ? w[i].db : db;
-    s.columns = columns_of(tile(w[0].da), db), s.slices = (db + s.columns - 1) / s.columns;
+    s.columns = columns_of(tile(w[0].da), db, q->envs * q->heads * count * ((db + 63) / 64)), s.slices = (db + s.columns - 1) / s.columns;
     s.items = (unsigned)(q->envs * q->heads) * s.count * s.slices;
-    int64_t segs = s.items >= 1024 ? 1 : 2048 / s.items, most = q->steps / 64;
+    int64_t segs = s.items >= FILL ? 1 : 2 * FILL / s.items, most = q->steps / 64;
     segs = segs < most ? segs : most;
     segs = segs < MAX_SEGS ? segs : MAX_SEGS;
     if (segs < 2) segs = 1;
