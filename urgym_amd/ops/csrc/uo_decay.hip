@@ -227,9 +227,75 @@ __device__ __forceinline__ void unit(float most, float* down, float* up) {
     *down = __uint_as_float(0x7f000000u - e);
 }
 
-// `by` times element (i, j) of the state that enters the sweep
-__device__ __forceinline__ float entering(const Sweep& w, unsigned nh, int i, int j, float by) {
-    return w.s_in && i < w.da && j < w.db ? by * w.s_in[(int64_t)nh * w.da * w.db + i * w.s_i + j * w.s_j] : 0.f;
+// element (i, j) of the state that enters the sweep
+__device__ __forceinline__ float entering(const Sweep& w, unsigned nh, int i, int j) {
+    return w.s_in && i < w.da && j < w.db ? w.in_mul * w.s_in[(int64_t)nh * w.da * w.db + i * w.s_i + j * w.s_j] : 0.f;
+}
+
+// All of a lane's elements of the state at p, unscaled, or to p: as vectors where its elements are neighbours (EXACT: then everything
+// exists and is 16-byte aligned).  p: the state of this (env, head).
+template <class L, int MODE>
+__device__ __forceinline__ void state_load(f4 (&S)[L::VA][L::VB], const Sweep& w, const float* p, int j0, int c, int g) {
+    constexpr int VA = L::VA, VB = L::VB;
+    if (MODE == EXACT && w.s_i == 1) {  // columns lie in a row: 4 neighbouring dimensions (16 bits), or all 4 VA of them
+#pragma unroll
+        for (int v = 0; v < VB; v++) {
+            const float* q = p + (int64_t)(j0 + L::col(v, c)) * w.s_j;
+#pragma unroll
+            for (int i = 0; i < VA; i++) {
+                f4 x = *(const f4*)(q + (L::ES == 2 ? L::dim(i, 4 * g) : 4 * VA * g + 4 * i));
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if (L::ES == 2) S[i][v][e] = x[e];
+                    else S[(4 * i + e) % VA][v][(4 * i + e) / VA] = x[e];
+                }
+            }
+        }
+    } else if (MODE == EXACT && L::ES == 4) {  // rows, of which a lane has VB neighbours
+        typedef float V __attribute__((ext_vector_type(VB)));
+#pragma unroll
+        for (int u = 0; u < VA; u++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                V x = *(const V*)(p + (int64_t)L::dim(u, 4 * g + r) * w.s_i + j0 + VB * c);
+#pragma unroll
+                for (int v = 0; v < VB; v++) S[u][v][r] = x[v];
+            }
+    } else {
+#pragma unroll
+        for (int u = 0; u < VA; u++)
+#pragma unroll
+            for (int v = 0; v < VB; v++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    int i = L::dim(u, 4 * g + r), j = j0 + L::col(v, c);
+                    S[u][v][r] = i < w.da && j < w.db ? p[(int64_t)i * w.s_i + (int64_t)j * w.s_j] : 0.f;
+                }
+    }
+}
+
+template <class L, int MODE>
+__device__ __forceinline__ void state_store(const f4 (&S)[L::VA][L::VB], float by, bool drop, const Sweep& w, float* p, int j0, int c, int g) {
+    constexpr int VA = L::VA, VB = L::VB;
+#pragma unroll
+    for (int u = 0; u < VA; u++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            int i = L::dim(u, 4 * g + r);
+            if (MODE == EXACT && L::ES == 4 && w.s_j == 1) {
+                typedef float V __attribute__((ext_vector_type(VB)));
+                V x;
+#pragma unroll
+                for (int v = 0; v < VB; v++) x[v] = drop ? 0.f : by * S[u][v][r];
+                *(V*)(p + (int64_t)i * w.s_i + j0 + VB * c) = x;
+            } else {
+#pragma unroll
+                for (int v = 0; v < VB; v++) {
+                    int j = j0 + L::col(v, c);
+                    if (i < w.da && j < w.db) p[(int64_t)i * w.s_i + (int64_t)j * w.s_j] = drop ? 0.f : by * S[u][v][r];
+                }
+            }
+        }
 }
 
 // element (r, u, v) of a wave's accumulators in ws: float4s, lane by lane
@@ -286,16 +352,8 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
 #pragma unroll
     for (int u = 0; u < VA; u++)
 #pragma unroll
-        for (int v = 0; v < VB; v++) {
-            if (STATE) {
-                S[u][v] = (f4)0.f;
-            } else if (all.segs > OWN_JOIN) {
-                S[u][v] = *held(all, item, VA * VB, u * VB + v, lane);
-            } else {
-#pragma unroll
-                for (int r = 0; r < 4; r++) S[u][v][r] = entering(w, nh, L::dim(u, 4 * g + r), j0 + L::col(v, c), 1.f);
-            }
-        }
+        for (int v = 0; v < VB; v++) S[u][v] = !STATE && all.segs > OWN_JOIN ? *held(all, item, VA * VB, u * VB + v, lane) : (f4)0.f;
+    if (!STATE && all.segs <= OWN_JOIN && w.s_in) state_load<L, MODE>(S, w, w.s_in + (int64_t)nh * da * db, j0, c, g);
     if (!STATE && all.segs <= OWN_JOIN) {
         for (unsigned before = seg; before; before--) {
             unsigned other = item - before * all.count * all.slices;
@@ -640,15 +698,7 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
     }
     if (!w.s_out || seg + 1 < all.segs) return;
     bool drop = w.s_drop && w.s_drop[n * w.start_sn];
-#pragma unroll
-    for (int u = 0; u < VA; u++)
-#pragma unroll
-        for (int v = 0; v < VB; v++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                int i = L::dim(u, 4 * g + r), j = j0 + L::col(v, c);
-                if (i < da && j < db) w.s_out[(int64_t)nh * da * db + i * w.s_i + j * w.s_j] = drop ? 0.f : w.out_mul * s_unit * S[u][v][r];
-            }
+    state_store<L, MODE>(S, w.out_mul * s_unit, drop, w, w.s_out + (int64_t)nh * da * db, j0, c, g);
 }
 
 // The states that the segments begin with, from what each adds: begin_0 = what enters, begin_{s+1} = left_s begin_s + added_s.
@@ -672,7 +722,7 @@ __global__ __launch_bounds__(256) void k_join(Sweeps all) {
     float left[PER];
     int g = lane / 16, c = lane % 16, u = tile / VB, v = tile % VB;
 #pragma unroll
-    for (int r = 0; r < 4; r++) begin[r] = entering(w, nh, L::dim(u, 4 * g + r), slice * 16 * VB + L::col(v, c), w.in_mul);
+    for (int r = 0; r < 4; r++) begin[r] = entering(w, nh, L::dim(u, 4 * g + r), slice * 16 * VB + L::col(v, c));
 #pragma unroll
     for (unsigned i = 0; i < PER; i++) {
         bool in = s0 + i < all.segs;
@@ -715,7 +765,8 @@ static void launch_tile(const Sweeps& s, hipStream_t st) {
         const Sweep& w = s.w[i];
         auto all = [&](int n) { return aligned(w.a, sizeof(T), n) && aligned(w.b, sizeof(T), n) && aligned(w.c, sizeof(T), n) && aligned(w.o, sizeof(T), n); };
         auto near = [](const Rows& r) { return (r.st < 0 ? -r.st : r.st) < ((int64_t)1 << 31) / ((int)sizeof(T) * L::CH); };  // 32-bit offsets
-        bool exact = w.da == L::DA && w.db % (16 * L::VB) == 0 && all(unit) && near(w.a) && near(w.b) && near(w.c);
+        bool exact = w.da == L::DA && w.db % (16 * L::VB) == 0 && all(unit) && near(w.a) && near(w.b) && near(w.c) &&
+                     (uintptr_t)w.s_in % 16 == 0 && (uintptr_t)w.s_out % 16 == 0;
         if (mode == EXACT && !exact) mode = FOURS;
         if (mode == FOURS && !(w.da % 4 == 0 && w.db % 4 == 0 && all(4))) mode = ANY;
     }
