@@ -51,7 +51,7 @@ def decay_bounds(args, kw, dtype):
     * In 32 bits: a sum of at most steps + 2 * 128 terms (u each, twice: products and sums), a power of the decay (an exponent
       of at most steps * |log_decay| rounded by u, the exponential by 2 u, once per step at the most: 4 u a step).
     * 16-bit inputs: the scores and the state inside a product are rounded to the type (u each, and one factor only in any
-      product), tokens that enter the state are held in two parts of the type (u^2).
+      product), tokens that enter the state are held in two parts of the type (u^2), three in bfloat16 (u^3).
     * The result is rounded to the type (states: float32)."""
     mags = decay_reference(*args, **kw, magnitude=True)
     refs = decay_reference(*args, **kw)
@@ -61,7 +61,7 @@ def decay_bounds(args, kw, dtype):
     out = []
     for i, (m, r) in enumerate(zip(mags, refs)):
         is_state = i in (1, 5)
-        inner = 0.0 if dtype == torch.float32 else 2 * u * u if is_state else 2 * u
+        inner = 0.0 if dtype == torch.float32 else 2 * u if not is_state else 2 * u ** (2 if dtype == torch.float16 else 3)
         out.append((n32 + inner) * m + (U32 if is_state else u) * r.abs() + 1e-30)
     return refs, out
 

@@ -575,8 +575,9 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
             }
         }
 
-        // the state: c weighted by its decay to the chunk's end.  In 16 bits the weighted value goes in as two parts of T, which
-        // keeps the state as exact as float32 sums of this length are.  S is touched only where the unit has become small, or, in
+        // the state: c weighted by its decay to the chunk's end.  In 16 bits the weighted value goes in as two parts of T (to 2^-16 in
+        // bf16: enough for o, less than its own rounding), and in bf16 as three where the state itself is an answer, in float32
+        // (forward, 500 x 1024 x 4 heads of 64: 261 us with two, 265 with three).  S is touched only where the unit has become small, or, in
         // fp16, where it does not bring this chunk's c into 2^6 .. 2^15, where both parts have their bits.
         float keep = n_tok < CH ? power(lg, n_tok) : whole, unit_new = s_unit * keep;
         bool off = unit_new < 1.f / 65536 || inside;
@@ -608,18 +609,25 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         for (int e = 0; e < FE; e++) by[e] = !inside || e / 4 * 16 + e % 4 + 4 * g >= last ? enter[e] * grow : 0.f;
 #pragma unroll
         for (int v = 0; v < VB; v++) {
-            Frag hi, lo;
+            Frag hi, lo, rest;
+            float z[FE];
 #pragma unroll
             for (int e = 0; e < FE; e++) {
                 float y = (float)fct[v][e] * by[e];
                 asm("" : "+v"(y));  // y is rounded here: its product fused into one of the conversions would give that another hi
-                hi[e] = (T)y;
-                if (HALF) lo[e] = (T)(y - (float)hi[e]);
+                hi[e] = (T)y, z[e] = y - (float)hi[e];
+                if (HALF) lo[e] = (T)z[e];
             }
 #pragma unroll
             for (int u = 0; u < VA; u++) {
                 S[u][v] = dot(S[u][v], fbt[u], hi);
                 if (HALF) S[u][v] = dot(S[u][v], fbt[u], lo);
+            }
+            if (HALF && !F16 && w.s_out) {
+#pragma unroll
+                for (int e = 0; e < FE; e++) rest[e] = (T)(z[e] - (float)lo[e]);
+#pragma unroll
+                for (int u = 0; u < VA; u++) S[u][v] = dot(S[u][v], fbt[u], rest);
             }
         }
         done();
