@@ -55,8 +55,11 @@ typedef struct {
     float scale;
 } urgym_ops_seq;
 
-/* float32 elements of workspace for urgym_ops_decay / urgym_ops_decay_backward (0: none needed, NULL may be passed; <0: error). */
-int64_t urgym_ops_decay_workspace(const urgym_ops_seq* s, int backward);
+/* The float32 elements of workspace (16-byte aligned) that urgym_ops_decay and urgym_ops_decay_backward need for these arguments (0:
+ * none, NULL may be passed; <0: error): for copies of tensors whose rows are not whole, aligned 16-byte vectors, and for the
+ * states of segments where few heads have many steps. */
+int64_t urgym_ops_decay_workspace(const urgym_ops_seq* s);
+int64_t urgym_ops_decay_backward_workspace(const urgym_ops_seq* s, const void* d_out, const int64_t d_out_stride[3]);
 
 /* S_t = exp(log_decay) S_{t-1} + k_t v_t^T (S_{t-1} = 0 where start_t), o_t = scale S_t^T q_t.
  * o [steps, envs, heads, dv], state_out float32 [envs, heads, dk, dv] (S of the last step), both contiguous. */

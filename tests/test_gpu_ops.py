@@ -463,14 +463,14 @@ def test_nothing_is_written_beyond_the_outputs(ops):
         sizes = [(35 * 3 * 2 * 40, dtype), (3 * 2 * 24 * 40, torch.float32), (35 * 3 * 2 * 24, dtype), (35 * 3 * 2 * 24, dtype),
                  (35 * 3 * 2 * 40, dtype), (3 * 2 * 24 * 40, torch.float32)]
         bufs = [framed(*z) for z in sizes]
-        n = [L.urgym_ops_decay_workspace(ctypes.byref(s), b) for b in (0, 1)]
+        stride = (ctypes.c_int64 * 3)(*do.stride()[:3])
+        n = [L.urgym_ops_decay_workspace(ctypes.byref(s)), L.urgym_ops_decay_backward_workspace(ctypes.byref(s), do.data_ptr(), stride)]
         ws = [framed(x, torch.float32) for x in n]
         at = [x[256:].data_ptr() for x in bufs]
         wat = [x[256:].data_ptr() if m else None for x, m in zip(ws, n)]
         stream = torch.cuda.current_stream().cuda_stream
         assert L.urgym_ops_decay(ctypes.byref(s), at[0], at[1], wat[0], stream) == 0
-        assert L.urgym_ops_decay_backward(ctypes.byref(s), do.data_ptr(), (ctypes.c_int64 * 3)(*do.stride()[:3]), dfinal.data_ptr(),
-                                          *at[2:], wat[1], stream) == 0
+        assert L.urgym_ops_decay_backward(ctypes.byref(s), do.data_ptr(), stride, dfinal.data_ptr(), *at[2:], wat[1], stream) == 0
         want = _grads(ops, q, k, v, g, state, start, do, dfinal, scale=0.2)
         for buf, y in zip(bufs, want):
             assert torch.equal(buf[256:-256], y.flatten()) and (buf[:256] == 7).all() and (buf[-256:] == 7).all()

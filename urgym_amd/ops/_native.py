@@ -10,7 +10,8 @@ LIB_PATH = os.path.join(_LIB, "liburgym_ops.so")
 TORCH_PATH = os.path.join(_LIB, "urgym_ops_torch.so")
 # C-ABI symbols declared in include/urgym_ops.h
 SYMBOLS = ["urgym_ops_last_error", "urgym_ops_layer_norm", "urgym_ops_layer_norm_workspace", "urgym_ops_layer_norm_backward",
-           "urgym_ops_decay_workspace", "urgym_ops_decay", "urgym_ops_decay_backward", "urgym_ops_decay_step"]
+           "urgym_ops_decay_workspace", "urgym_ops_decay_backward_workspace", "urgym_ops_decay",
+            "urgym_ops_decay_backward", "urgym_ops_decay_step"]
 F32, BF16, F16 = 0, 1, 2
 MAX_HEAD_DIM = 128
 _lib = None
@@ -44,8 +45,9 @@ def lib():
         L.urgym_ops_layer_norm_workspace.argtypes = [Q, Q]
         L.urgym_ops_layer_norm_workspace.restype = Q
         L.urgym_ops_layer_norm_backward.argtypes = [I, I, Q, Q, P, Q, P, Q, P, P, P, P, P, P, P, P]
-        L.urgym_ops_decay_workspace.argtypes = [ctypes.POINTER(Seq), I]
-        L.urgym_ops_decay_workspace.restype = Q
+        L.urgym_ops_decay_workspace.argtypes = [ctypes.POINTER(Seq)]
+        L.urgym_ops_decay_backward_workspace.argtypes = [ctypes.POINTER(Seq), P, Q * 3]
+        L.urgym_ops_decay_workspace.restype = L.urgym_ops_decay_backward_workspace.restype = Q
         L.urgym_ops_decay.argtypes = [ctypes.POINTER(Seq), P, P, P, P]
         L.urgym_ops_decay_backward.argtypes = [ctypes.POINTER(Seq), P, Q * 3, P, P, P, P, P, P, P]
         L.urgym_ops_decay_step.argtypes = [I, Q, I, I, I, P, Q, Q, P, Q, Q, P, Q, Q, P, P, Q, F, P, P, P, P]

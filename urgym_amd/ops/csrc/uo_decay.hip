@@ -128,44 +128,63 @@ __device__ __forceinline__ f4 dot(f4 acc, f4 a, f4 b) {
 // 2^(lg n); 1 for n = 0, whatever lg
 __device__ __forceinline__ float power(float lg, int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(lg * (float)n); }
 
-// How rows are fetched.  EXACT: widths are the tiles', everything is 16-byte aligned and a chunk lies within 2 GiB: from memory into
-// LDS directly.  Otherwise through registers, 4 elements at a time where widths and offsets are multiples of 4 (FOURS), or one (ANY).
-enum { EXACT, FOURS, ANY };
+// N elements at an address that need not be a vector's
+template <typename T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Piece {
+    T __attribute__((ext_vector_type(N))) v;
+};
 
-// 16 bytes of elements as words, from column col of a row of `width` elements at p.  Columns that do not exist are read as the last
-// one (no branch holds up the loads after it); `present` zeroes them afterwards.
-template <typename T, int MODE>
-__device__ __forceinline__ void fetch(unsigned* to, const T* p, int col, int width) {
-    constexpr int N = 16 / sizeof(T);
-    if constexpr (MODE == FOURS) {
-        typedef unsigned V __attribute__((ext_vector_type(sizeof(T))));
-#pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            V x = *(const V*)(p + (col + i < width ? col + i : width - 4));
-#pragma unroll
-            for (int e = 0; e < (int)sizeof(T); e++) to[i * (int)sizeof(T) / 4 + e] = x[e];
-        }
-    } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < N; i++) to[i] = ((const unsigned*)p)[col + i < width ? col + i : width - 1];
-    } else {
-        unsigned x[N];
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] = ((const uint16_t*)p)[col + i < width ? col + i : width - 1];
-#pragma unroll
-        for (int i = 0; i < 4; i++) to[i] = x[2 * i] | x[2 * i + 1] << 16;
-    }
-}
-
+// Columns col .. of the row of `width` elements at p as 16 bytes, zeros where they do not exist.  A piece that leaves the row is the
+// row's last 16 bytes, moved to their places; in rows of less than that each element is clamped.
 template <typename T>
-__device__ __forceinline__ u4 present(const unsigned* from, int col, int width) {
+__device__ __forceinline__ u4 padded(const T* p, int col, int width) {
+    constexpr int N = 16 / sizeof(T);
     u4 x;
+    if (width >= N) {
+        x = __builtin_bit_cast(u4, ((const Piece<T, N>*)(p + (col < width - N ? col : width - N)))->v);
+        int over = col - (width - N);  // elements to move down by
+        if (over >= N) return (u4)0u;
+        over = over < 0 ? 0 : over;
+        if (over & (N / 2)) x = u4{x[2], x[3], 0u, 0u};
+        if (over & (N / 4)) x = u4{x[1], x[2], x[3], 0u};
+        if (N == 8 && (over & 1)) x = u4{x[0] >> 16 | x[1] << 16, x[1] >> 16 | x[2] << 16, x[2] >> 16 | x[3] << 16, x[3] >> 16};
+        return x;
+    }
+    T y[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) y[i] = p[col + i < width ? col + i : width - 1];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        if constexpr (sizeof(T) == 4) x[i] = col + i < width ? from[i] : 0u;
-        else x[i] = from[i] & ((col + 2 * i < width ? 0xffffu : 0u) | (col + 2 * i + 1 < width ? 0xffff0000u : 0u));
+        if constexpr (sizeof(T) == 4) x[i] = col + i < width ? __builtin_bit_cast(unsigned, y[i]) : 0u;
+        else x[i] = (col + 2 * i < width ? __builtin_bit_cast(uint16_t, y[2 * i]) : 0u) | (col + 2 * i + 1 < width ? (unsigned)__builtin_bit_cast(uint16_t, y[2 * i + 1]) << 16 : 0u);
     }
     return x;
+}
+
+// Tensors whose rows the sweeps cannot load as aligned vectors (odd widths, odd addresses, a chunk over more than 2 GiB) are first
+// copied, rows padded to whole vectors: it costs their bytes three times, but the sweep then runs at its full rate (65 wide heads,
+// bf16, 103 x 1151 x 8: forward 3.2 ms with rows fetched through registers in the sweep).
+struct Packs {
+    struct {
+        Rows from;
+        void* to;
+        int width;
+    } t[4];
+    int count;
+    unsigned heads, envs;
+    int64_t steps;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_pack(Packs p) {
+    constexpr int N = 16 / sizeof(T);
+    const auto& w = p.t[blockIdx.z];
+    const unsigned pieces = (w.width + N - 1) / N, i = blockIdx.x * 256 + threadIdx.x, row = i / pieces, n = row / p.heads, h = row % p.heads;
+    if (n >= p.envs) return;
+    const int col = i % pieces * N;
+    const T* from = (const T*)w.from.p + n * w.from.sn + h * w.from.sh;
+    u4* to = (u4*)w.to + i;
+    for (int64_t t = blockIdx.y; t < p.steps; t += gridDim.y) to[t * p.envs * p.heads * pieces] = padded(from + t * w.from.st, col, w.width);
 }
 
 // 16 bytes at base + each lane's offset to LDS bytes to .. to + 1023, lane by lane.  Written as assembly because the compiler would
@@ -232,12 +251,18 @@ __device__ __forceinline__ float entering(const Sweep& w, unsigned nh, int i, in
     return w.s_in && i < w.da && j < w.db ? w.in_mul * w.s_in[(int64_t)nh * w.da * w.db + i * w.s_i + j * w.s_j] : 0.f;
 }
 
-// All of a lane's elements of the state at p, unscaled, or to p: as vectors where its elements are neighbours (EXACT: then everything
-// exists and is 16-byte aligned).  p: the state of this (env, head).
-template <class L, int MODE>
+// All of a lane's elements of the state at p, unscaled, or to p: as vectors where its elements are neighbours, the tiles are full and p
+// is 16-byte aligned.  p: the state of this (env, head).
+template <class L>
+__device__ __forceinline__ bool vectors(const Sweep& w, const float* p) {
+    return w.da == L::DA && w.db % (16 * L::VB) == 0 && (uintptr_t)p % 16 == 0;
+}
+
+template <class L>
 __device__ __forceinline__ void state_load(f4 (&S)[L::VA][L::VB], const Sweep& w, const float* p, int j0, int c, int g) {
     constexpr int VA = L::VA, VB = L::VB;
-    if (MODE == EXACT && w.s_i == 1) {  // columns lie in a row: 4 neighbouring dimensions (16 bits), or all 4 VA of them
+    const bool full = vectors<L>(w, p);
+    if (full && w.s_i == 1) {  // columns lie in a row: 4 neighbouring dimensions (16 bits), or all 4 VA of them
 #pragma unroll
         for (int v = 0; v < VB; v++) {
             const float* q = p + (int64_t)(j0 + L::col(v, c)) * w.s_j;
@@ -251,7 +276,7 @@ __device__ __forceinline__ void state_load(f4 (&S)[L::VA][L::VB], const Sweep& w
                 }
             }
         }
-    } else if (MODE == EXACT && L::ES == 4) {  // rows, of which a lane has VB neighbours
+    } else if (full && L::ES == 4) {  // rows, of which a lane has VB neighbours
         typedef float V __attribute__((ext_vector_type(VB)));
 #pragma unroll
         for (int u = 0; u < VA; u++)
@@ -274,15 +299,16 @@ __device__ __forceinline__ void state_load(f4 (&S)[L::VA][L::VB], const Sweep& w
     }
 }
 
-template <class L, int MODE>
+template <class L>
 __device__ __forceinline__ void state_store(const f4 (&S)[L::VA][L::VB], float by, bool drop, const Sweep& w, float* p, int j0, int c, int g) {
     constexpr int VA = L::VA, VB = L::VB;
+    const bool full = L::ES == 4 && w.s_j == 1 && vectors<L>(w, p);
 #pragma unroll
     for (int u = 0; u < VA; u++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             int i = L::dim(u, 4 * g + r);
-            if (MODE == EXACT && L::ES == 4 && w.s_j == 1) {
+            if (full) {
                 typedef float V __attribute__((ext_vector_type(VB)));
                 V x;
 #pragma unroll
@@ -309,7 +335,7 @@ __device__ __forceinline__ f4 joined(f4 x, float left, f4 add) { return left == 
 // STATE: only what the segment adds to the state (no a, no o); segments after it need that before they can begin.
 // Two waves a SIMD at least, that is 256 registers at most: then matrix instructions accumulate in ordinary registers, where C is
 // scaled and converted between any two of them.
-template <typename T, class L, int MODE, bool STATE>
+template <typename T, class L, bool STATE>
 __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
     typedef typename FragOf<T>::type Frag;
     constexpr int FE = L::FE, NB = L::NB, CH = L::CH, NF = L::NF, VA = L::VA, VB = L::VB, RA = L::RA, RC = L::RC;
@@ -353,7 +379,7 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
     for (int u = 0; u < VA; u++)
 #pragma unroll
         for (int v = 0; v < VB; v++) S[u][v] = !STATE && all.segs > OWN_JOIN ? *held(all, item, VA * VB, u * VB + v, lane) : (f4)0.f;
-    if (!STATE && all.segs <= OWN_JOIN && w.s_in) state_load<L, MODE>(S, w, w.s_in + (int64_t)nh * da * db, j0, c, g);
+    if (!STATE && all.segs <= OWN_JOIN && w.s_in) state_load<L>(S, w, w.s_in + (int64_t)nh * da * db, j0, c, g);
     if (!STATE && all.segs <= OWN_JOIN) {
         for (unsigned before = seg; before; before--) {
             unsigned other = item - before * all.count * all.slices;
@@ -387,50 +413,33 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         return n_tok;
     };
 
-    // A chunk's rows into LDS: `issue`, then `commit`, which waits (or writes what passes through registers).  Lane by lane 16 bytes; the rows before a short chunk's are its first one's, zeroed before they are used.
-    constexpr int KA = CH * RA / 1024, KC = CH * RC / 1024;
-    unsigned stage[MODE == EXACT ? 1 : 2 * KA + KC][4];
+    // A chunk's rows into LDS, lane by lane 16 bytes; the rows before a short chunk's are its first one's, zeroed before they are used.
+    // What lies beyond a row's last vector is not loaded and stays zero.  Offsets are unsigned: from a load's lowest row, which in
+    // a backward sweep is the last.
     const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-    auto rows_of = [&](auto size, auto part, int k0, const T* base, int64_t st, int tile0, int width, int x, int n_tok) {
-        constexpr int RB = decltype(size)::value, K = decltype(part)::value, ROWS = 1024 / RB;  // rows of one load
+    auto load_rows = [&](auto size, auto whole, const T* base, int64_t st, int tile0, int width, int x, int n_tok) {
+        constexpr int RB = decltype(size)::value, K = CH * RB / 1024, ROWS = 1024 / RB;  // rows of one load
         const int l = lane / (RB / 16);
+        const unsigned stride = (unsigned)(st < 0 ? -st : st) * sizeof(T);
 #pragma unroll
         for (int k = 0; k < K; k++) {
             int t = k * ROWS + l, ts = ROWS % 8 ? t : l;
             int byte = place<RB>(ts, lane * 16 % RB) - ts * RB;  // exchanging blocks twice is nothing: what belongs at this place
             int tt = n_tok == CH ? t : t < CH - n_tok ? 0 : t - (CH - n_tok);
-            if constexpr (MODE == EXACT) {  // offsets are unsigned: from the load's lowest row, the last one of a backward sweep
-                unsigned size = (unsigned)(st < 0 ? -st : st) * sizeof(T);
-                int low = n_tok == CH ? k * ROWS : 0, row = n_tok == CH ? l : tt, last = n_tok == CH ? ROWS - 1 : n_tok - 1;
-                const T* from = base + (int64_t)(x + low + (st < 0 ? last : 0)) * st;
-                load_to_lds(at + tile0 + k * 1024, from, (unsigned)(st < 0 ? last - row : row) * size + byte);
-            } else {
-                fetch<T, MODE>(stage[k0 + k], base + (int64_t)(x + tt) * st, byte / (int)sizeof(T), width);
-            }
+            int low = n_tok == CH ? k * ROWS : 0, row = n_tok == CH ? l : tt, last = n_tok == CH ? ROWS - 1 : n_tok - 1;
+            const T* from = base + (int64_t)(x + low + (st < 0 ? last : 0)) * st;
+            if (decltype(whole)::value || byte < width * (int)sizeof(T)) load_to_lds(at + tile0 + k * 1024, from, (unsigned)(st < 0 ? last - row : row) * stride + byte);
         }
+    };
+    auto rows_of = [&](auto size, const T* base, int64_t st, int tile0, int width, int x, int n_tok) {
+        if (width * (int)sizeof(T) >= decltype(size)::value) load_rows(size, Int<1>(), base, st, tile0, width, x, n_tok);
+        else load_rows(size, Int<0>(), base, st, tile0, width, x, n_tok);
     };
     auto issue = [&](int x, int n_tok) {
-        if (MODE == EXACT) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every read has been answered
-        if (!STATE) rows_of(Int<RA>(), Int<KA>(), 0, pa, sta, L::A0, da, x, n_tok);
-        rows_of(Int<RA>(), Int<KA>(), KA, pb, stb, L::B0, da, x, n_tok);
-        rows_of(Int<RC>(), Int<KC>(), 2 * KA, pc, stc, L::C0, db - j0, x, n_tok);
-    };
-    auto commit = [&] {
-        if constexpr (MODE == EXACT) {
-            landed();
-        } else {
-            auto put = [&](auto size, auto part, int k0, int tile0, int width) {
-                constexpr int RB = decltype(size)::value, K = decltype(part)::value, ROWS = 1024 / RB;
-#pragma unroll
-                for (int k = 0; k < K; k++) {
-                    int l = lane / (RB / 16), ts = ROWS % 8 ? k * ROWS + l : l, byte = place<RB>(ts, lane * 16 % RB) - ts * RB;
-                    *(u4*)(lds + tile0 + k * 1024 + lane * 16) = present<T>(stage[k0 + k], byte / (int)sizeof(T), width);
-                }
-            };
-            if (!STATE) put(Int<RA>(), Int<KA>(), 0, L::A0, da);
-            put(Int<RA>(), Int<KA>(), KA, L::B0, da);
-            put(Int<RC>(), Int<KC>(), 2 * KA, L::C0, db - j0);
-        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every read has been answered
+        if (!STATE) rows_of(Int<RA>(), pa, sta, L::A0, da, x, n_tok);
+        rows_of(Int<RA>(), pb, stb, L::B0, da, x, n_tok);
+        rows_of(Int<RC>(), pc, stc, L::C0, db - j0, x, n_tok);
     };
 
     // One chunk: the operands from LDS, then (`next`: the next chunk's loads begin) o and the state, then (`done`: they have landed)
@@ -640,17 +649,22 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
 #pragma unroll
                     for (int q = 0; q < 4 * VB / RUN; q++) {
                         int left = db - j0 - RUN * g - 32 * q;
-                        constexpr int N = MODE == EXACT ? 16 / sizeof(T) : MODE == FOURS ? 4 : 1;
-                        typedef T V __attribute__((ext_vector_type(N)));
+                        constexpr int N = 16 / sizeof(T);
 #pragma unroll
                         for (int e = 0; e < RUN; e += N) {
-                            V y;
+                            Piece<T, N> y;
 #pragma unroll
                             for (int i = 0; i < N; i++) {
                                 int v = HALF ? 2 * q + (e + i) / 4 : (e + i) % VB, r = HALF ? (e + i) % 4 : (e + i) / VB;
-                                y[i] = (T)(F16 ? O[it][v][r] * p_up : O[it][v][r]);
+                                y.v[i] = (T)(F16 ? O[it][v][r] * p_up : O[it][v][r]);
                             }
-                            if (MODE == EXACT || e < left) *(V*)(to + 32 * q + e) = y;
+                            if (e + N <= left) {
+                                *(Piece<T, N>*)(to + 32 * q + e) = y;
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < N; i++)
+                                    if (e + i < left) to[32 * q + e + i] = y.v[i];
+                            }
                         }
                     }
                 }
@@ -658,6 +672,8 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         return true;
     };
 
+    if (da < L::DA || db - j0 < 16 * VB)
+        for (int i = lane * 16; i < L::BUF; i += 1024) *(u4*)(lds + i) = (u4)0u;
     bool fresh;
     unsigned inside;
     int n_tok = chunk(0, &fresh, &inside);
@@ -673,7 +689,7 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
 #pragma unroll
     for (int b = 0; b < NB; b++) carry[b] = w.sa * power(lg, 16 * b + c + w.e0);
     whole = power(lg, CH);
-    commit();
+    landed();
     for (int x = 0; x < steps;) {
         const int x_next = x + n_tok;
         bool f_next = false;
@@ -682,11 +698,11 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         auto begin = [&] {
             if (n_next) issue(x_next, n_next);
         };
-        if (!compute(x, n_tok, fresh, inside, begin, commit)) {
+        if (!compute(x, n_tok, fresh, inside, begin, landed)) {
             (inside ? cut : slow) = x_next;
             n_tok = chunk(x, &fresh, &inside);
             issue(x, n_tok);
-            commit();
+            landed();
             continue;
         }
         x = x_next, n_tok = n_next, fresh = f_next, inside = i_next;
@@ -706,7 +722,7 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
     }
     if (!w.s_out || seg + 1 < all.segs) return;
     bool drop = w.s_drop && w.s_drop[n * w.start_sn];
-    state_store<L, MODE>(S, w.out_mul * s_unit, drop, w, w.s_out + (int64_t)nh * da * db, j0, c, g);
+    state_store<L>(S, w.out_mul * s_unit, drop, w, w.s_out + (int64_t)nh * da * db, j0, c, g);
 }
 
 // The states that the segments begin with, from what each adds: begin_0 = what enters, begin_{s+1} = left_s begin_s + added_s.
@@ -761,35 +777,16 @@ constexpr int64_t FILL = 1024;  // waves: one for each SIMD
 // waves fill the chip (with fewer, the time of one wave's chunk counts).
 static int columns_of(int tile, int db, int64_t waves) { return tile == 64 && db > 32 && waves >= FILL ? 64 : 32; }
 
-// every access of the tensor falls on multiples of `elements` elements
-static bool aligned(const Rows& r, int size, int elements) {
-    return (uintptr_t)r.p % (size * elements) == 0 && r.st % elements == 0 && r.sn % elements == 0 && r.sh % elements == 0;
-}
-
 template <typename T, class L>
 static void launch_tile(const Sweeps& s, hipStream_t st) {
-    int mode = EXACT, unit = 16 / sizeof(T);
-    for (unsigned i = 0; i < s.count; i++) {
-        const Sweep& w = s.w[i];
-        auto all = [&](int n) { return aligned(w.a, sizeof(T), n) && aligned(w.b, sizeof(T), n) && aligned(w.c, sizeof(T), n) && aligned(w.o, sizeof(T), n); };
-        auto near = [](const Rows& r) { return (r.st < 0 ? -r.st : r.st) < ((int64_t)1 << 31) / ((int)sizeof(T) * L::CH); };  // 32-bit offsets
-        bool exact = w.da == L::DA && w.db % (16 * L::VB) == 0 && all(unit) && near(w.a) && near(w.b) && near(w.c) &&
-                     (uintptr_t)w.s_in % 16 == 0 && (uintptr_t)w.s_out % 16 == 0;
-        if (mode == EXACT && !exact) mode = FOURS;
-        if (mode == FOURS && !(w.da % 4 == 0 && w.db % 4 == 0 && all(4))) mode = ANY;
-    }
     unsigned grid = (s.items + 7) / 8 * 8;
     if (s.segs > 1) {
-        if (mode == EXACT) k_sweep<T, L, EXACT, true><<<grid, 64, 0, st>>>(s);
-        else if (mode == FOURS) k_sweep<T, L, FOURS, true><<<grid, 64, 0, st>>>(s);
-        else k_sweep<T, L, ANY, true><<<grid, 64, 0, st>>>(s);
+        k_sweep<T, L, true><<<grid, 64, 0, st>>>(s);
         unsigned parts = s.items / s.segs * L::VA * L::VB * 2;
         if (s.segs > 4 * RUNS) k_join<L, 16><<<parts, 256, 0, st>>>(s);
         else if (s.segs > OWN_JOIN) k_join<L, 4><<<parts, 256, 0, st>>>(s);
     }
-    if (mode == EXACT) k_sweep<T, L, EXACT, false><<<grid, 64, 0, st>>>(s);
-    else if (mode == FOURS) k_sweep<T, L, FOURS, false><<<grid, 64, 0, st>>>(s);
-    else k_sweep<T, L, ANY, false><<<grid, 64, 0, st>>>(s);
+    k_sweep<T, L, false><<<grid, 64, 0, st>>>(s);
 }
 
 template <typename T>
@@ -822,7 +819,8 @@ static Sweeps plan(const urgym_ops_seq* q, const Sweep* w, int count) {
     return s;
 }
 
-static int64_t workspace(const Sweeps& s) { return s.segs > 1 ? (int64_t)s.items * (tile(s.w[0].da) * s.columns + 1) : 0; }
+// in floats, whole vectors
+static int64_t workspace(const Sweeps& s) { return s.segs > 1 ? ((int64_t)s.items * (tile(s.w[0].da) * s.columns + 1) + 3) / 4 * 4 : 0; }
 
 static void launch(const urgym_ops_seq* q, Sweeps s, float* ws, hipStream_t st) {
     s.ws = ws, s.left = ws + (int64_t)s.items * tile(s.w[0].da) * s.columns;
@@ -977,50 +975,81 @@ static Sweep backward(const urgym_ops_seq* s, Rows a, Rows b, Rows c, Rows o, in
     return w;
 }
 
-// the launches of one direction: o's, or those of dk, dq and dv, which read the same rows and share a launch where their tiles agree
-static int plans(const urgym_ops_seq* s, Rows o, Sweeps* p) {
-    Sweep w = forward(s, rows(s->q, s->q_stride), rows(s->k, s->k_stride), rows(s->v, s->v_stride), o, s->dk, s->dv, false);
-    p[0] = plan(s, &w, 1);
-    return 1;
+// what the sweeps read of r: itself, or (padded rows, appended to the workspace at `floats`) its copy
+static Rows readable(const urgym_ops_seq* s, Rows r, int d, float* ws, int64_t* floats, Packs* p) {
+    int size = s->dtype == URGYM_OPS_F32 ? 4 : 2, n = 16 / size, width = (d + n - 1) / n * n;
+    bool far = (r.st < 0 ? -r.st : r.st) >= ((int64_t)1 << 31) / (32 * size);
+    if (d % n == 0 && (uintptr_t)r.p % 16 == 0 && r.st % n == 0 && r.sn % n == 0 && r.sh % n == 0 && !far) return r;
+    Rows to = {ws + *floats, s->envs * s->heads * width, (int64_t)s->heads * width, width};
+    p->t[p->count++] = {r, (void*)to.p, d};
+    *floats += s->steps * s->envs * s->heads * width * size / 4;
+    return to;
 }
 
-static int plans(const urgym_ops_seq* s, Rows g, const float* d_state_out, void* dq, void* dk, void* dv, float* d_state, Sweeps* p) {
-    Rows q = rows(s->q, s->q_stride), k = rows(s->k, s->k_stride), v = rows(s->v, s->v_stride);
-    Sweep w[3] = {backward(s, v, g, q, packed(dk, s, s->dk), s->dv, s->dk, true, d_state_out),
-                  forward(s, g, v, k, packed(dq, s, s->dk), s->dv, s->dk, true),
-                  backward(s, k, q, g, packed(dv, s, s->dv), s->dk, s->dv, false, d_state_out)};
-    w[2].s_out = d_state;
-    if (tile(s->dk) == tile(s->dv)) {
-        p[0] = plan(s, w, 3);
-        return 1;
+// Everything one direction enqueues, and its workspace: copies of what cannot be read as it is, then the launches of o's sweep, or
+// of those of dk, dq and dv, which read the same rows and share a launch where their tiles agree.
+struct Work {
+    Packs packs;
+    Sweeps sweeps[2];
+    int count;
+    float* ws;         // of the sweeps
+    int64_t floats;    // in all
+};
+
+static Work work(const urgym_ops_seq* s, const Rows* g, float* ws) {
+    Work w = {};
+    w.packs.heads = s->heads, w.packs.envs = (unsigned)s->envs, w.packs.steps = s->steps;
+    Rows q = readable(s, rows(s->q, s->q_stride), s->dk, ws, &w.floats, &w.packs), k = readable(s, rows(s->k, s->k_stride), s->dk, ws, &w.floats, &w.packs),
+         v = readable(s, rows(s->v, s->v_stride), s->dv, ws, &w.floats, &w.packs);
+    Rows none = {};
+    if (!g) {
+        Sweep o = forward(s, q, k, v, none, s->dk, s->dv, false);
+        w.sweeps[w.count++] = plan(s, &o, 1);
+    } else {
+        Rows d = readable(s, *g, s->dv, ws, &w.floats, &w.packs);
+        Sweep b[3] = {backward(s, v, d, q, none, s->dv, s->dk, true, nullptr), forward(s, d, v, k, none, s->dv, s->dk, true),
+                      backward(s, k, q, d, none, s->dk, s->dv, false, nullptr)};
+        if (tile(s->dk) == tile(s->dv)) w.sweeps[w.count++] = plan(s, b, 3);
+        else w.sweeps[w.count++] = plan(s, b, 2), w.sweeps[w.count++] = plan(s, b + 2, 1);
     }
-    p[0] = plan(s, w, 2), p[1] = plan(s, w + 2, 1);
-    return 2;
-}
-
-extern "C" int64_t urgym_ops_decay_workspace(const urgym_ops_seq* s, int backward) {
-    if (seq_check("urgym_ops_decay_workspace", s)) return -1;
-    Sweeps p[2];
+    w.ws = ws + w.floats;
     int64_t most = 0;
-    for (int i = 0, n = backward ? plans(s, Rows{}, nullptr, nullptr, nullptr, nullptr, nullptr, p) : plans(s, Rows{}, p); i < n; i++)
-        most = workspace(p[i]) > most ? workspace(p[i]) : most;
-    return most;
+    for (int i = 0; i < w.count; i++) most = workspace(w.sweeps[i]) > most ? workspace(w.sweeps[i]) : most;
+    w.floats += most;
+    return w;
 }
 
-static int run(const char* what, const urgym_ops_seq* s, const Sweeps* p, int n, float* ws, hipStream_t st) {
-    for (int i = 0; i < n; i++)
-        if (workspace(p[i]) && !ws) return uo_fail("%s: a workspace is needed", what);
-    for (int i = 0; i < n; i++) launch(s, p[i], ws, st);
+extern "C" int64_t urgym_ops_decay_workspace(const urgym_ops_seq* s) {
+    if (seq_check("urgym_ops_decay_workspace", s)) return -1;
+    return work(s, nullptr, nullptr).floats;
+}
+
+extern "C" int64_t urgym_ops_decay_backward_workspace(const urgym_ops_seq* s, const void* d_out, const int64_t d_out_stride[3]) {
+    if (seq_check("urgym_ops_decay_backward_workspace", s)) return -1;
+    if (!d_out_stride) return uo_fail("urgym_ops_decay_backward_workspace: d_out's strides are needed");
+    Rows g = rows(d_out, d_out_stride);
+    return work(s, &g, nullptr).floats;
+}
+
+static int run(const char* what, const urgym_ops_seq* s, const Work& w, hipStream_t st) {
+    if (w.packs.count) {
+        int size = s->dtype == URGYM_OPS_F32 ? 4 : 2, n = 16 / size;
+        int64_t pieces = (int64_t)s->envs * s->heads * (((s->dk > s->dv ? s->dk : s->dv) + n - 1) / n);
+        dim3 grid((unsigned)((pieces + 255) / 256), (unsigned)(s->steps < 65535 ? s->steps : 65535), w.packs.count);
+        if (s->dtype == URGYM_OPS_F32) k_pack<float><<<grid, 256, 0, st>>>(w.packs);
+        else k_pack<f16><<<grid, 256, 0, st>>>(w.packs);
+    }
+    for (int i = 0; i < w.count; i++) launch(s, w.sweeps[i], w.ws, st);
     return uo_launched(what);
 }
 
 extern "C" int urgym_ops_decay(const urgym_ops_seq* s, void* o, float* state_out, float* ws, void* stream) {
     if (seq_check("urgym_ops_decay", s)) return -1;
     if (!o || !state_out) return uo_fail("urgym_ops_decay: o and state_out are needed");
-    Sweeps p[1];
-    int n = plans(s, packed(o, s, s->dv), p);
-    p[0].w[0].s_out = state_out;
-    return run("urgym_ops_decay", s, p, n, ws, (hipStream_t)stream);
+    Work w = work(s, nullptr, ws);
+    if (w.floats && (!ws || (uintptr_t)ws % 16)) return uo_fail("urgym_ops_decay: a workspace is needed, 16-byte aligned");
+    w.sweeps[0].w[0].o = packed(o, s, s->dv), w.sweeps[0].w[0].s_out = state_out;
+    return run("urgym_ops_decay", s, w, (hipStream_t)stream);
 }
 
 extern "C" int urgym_ops_decay_backward(const urgym_ops_seq* s, const void* d_out, const int64_t d_out_stride[3],
@@ -1028,9 +1057,13 @@ extern "C" int urgym_ops_decay_backward(const urgym_ops_seq* s, const void* d_ou
                                         void* stream) {
     if (seq_check("urgym_ops_decay_backward", s)) return -1;
     if (!d_out || !d_out_stride || !dq || !dk || !dv) return uo_fail("urgym_ops_decay_backward: d_out, dq, dk and dv are needed");
-    Sweeps p[2];
-    int n = plans(s, rows(d_out, d_out_stride), d_state_out, dq, dk, dv, d_state, p);
-    return run("urgym_ops_decay_backward", s, p, n, ws, (hipStream_t)stream);
+    Rows g = rows(d_out, d_out_stride);
+    Work w = work(s, &g, ws);
+    if (w.floats && (!ws || (uintptr_t)ws % 16)) return uo_fail("urgym_ops_decay_backward: a workspace is needed, 16-byte aligned");
+    Sweep &k = w.sweeps[0].w[0], &q = w.sweeps[0].w[1], &v = w.count == 1 ? w.sweeps[0].w[2] : w.sweeps[1].w[0];
+    k.o = reversed(packed(dk, s, s->dk), s), q.o = packed(dq, s, s->dk), v.o = reversed(packed(dv, s, s->dv), s);
+    k.s_in = v.s_in = d_state_out, v.s_out = d_state;
+    return run("urgym_ops_decay_backward", s, w, (hipStream_t)stream);
 }
 
 extern "C" int urgym_ops_decay_step(int dtype, int64_t envs, int heads, int dk, int dv, const void* q, int64_t q_sn, int64_t q_sh,

@@ -179,10 +179,9 @@ static urgym_ops_seq sequence(const Tensor& q, const Tensor& k, const Tensor& v,
     return s;
 }
 
-static Tensor workspace(const urgym_ops_seq& s, bool backward, const Tensor& q) {
-    int64_t n = urgym_ops_decay_workspace(&s, backward);
-    TORCH_CHECK(n >= 0, urgym_ops_last_error());
-    return n ? at::empty({n}, q.options().dtype(at::kFloat)) : Tensor();
+static Tensor workspace(int64_t floats, const Tensor& q) {
+    TORCH_CHECK(floats >= 0, urgym_ops_last_error());
+    return floats ? at::empty({floats}, q.options().dtype(at::kFloat)) : Tensor();
 }
 
 static std::tuple<Tensor, Tensor> decay_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state,
@@ -192,7 +191,7 @@ static std::tuple<Tensor, Tensor> decay_forward(const Tensor& q, const Tensor& k
     Tensor final = at::empty({q.size(1), q.size(2), q.size(3), v.size(3)}, q.options().dtype(at::kFloat));
     if (q.size(1)) {
         urgym_ops_seq s = sequence(q, k, v, log_decay, state, start, scale);
-        Tensor ws = workspace(s, false, q);
+        Tensor ws = workspace(urgym_ops_decay_workspace(&s), q);
         done(urgym_ops_decay(&s, o.mutable_data_ptr(), final.mutable_data_ptr<float>(), (float*)ptr(ws), stream_of(q)));
     }
     return {o, final};
@@ -221,8 +220,8 @@ struct DecayAttention : torch::autograd::Function<DecayAttention> {
             Tensor d_out = grads[0].defined() ? rows(grads[0]) : at::zeros(v.sizes(), v.options());
             Tensor d_final = grads[1].defined() ? grads[1].contiguous() : Tensor();
             urgym_ops_seq s = sequence(q, k, v, log_decay, state, start, ctx->saved_data["scale"].toDouble());
-            Tensor ws = workspace(s, true, q);
             int64_t stride[3] = {d_out.stride(0), d_out.stride(1), d_out.stride(2)};
+            Tensor ws = workspace(urgym_ops_decay_backward_workspace(&s, d_out.const_data_ptr(), stride), q);
             done(urgym_ops_decay_backward(&s, d_out.const_data_ptr(), stride, (const float*)ptr(d_final), dq.mutable_data_ptr(), dk.mutable_data_ptr(),
                                           dv.mutable_data_ptr(), (float*)ptr(dstate), (float*)ptr(ws), stream_of(q)));
         }
