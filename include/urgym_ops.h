@@ -22,6 +22,7 @@ extern "C" {
 #define URGYM_OPS_BF16 1
 #define URGYM_OPS_F16 2
 #define URGYM_OPS_MAX_HEAD_DIM 128
+#define URGYM_OPS_MAX_HEADS (1 << 22) /* envs * heads in one call; steps: up to 1 << 30 */
 
 /* Message of this thread's last failed call. */
 const char* urgym_ops_last_error(void);

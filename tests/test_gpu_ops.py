@@ -81,6 +81,17 @@ def test_long_axis_with_few_heads(ops, dtype):
 
 
 @pytest.mark.parametrize("dtype", ALL, ids=str)
+def test_very_long_axis(ops, dtype):
+    """over 32 pieces of the axis, whose states are joined in longer runs"""
+    q, k, v, g, state, _, do, dfinal = _case(5003, 1, 2, 17, 32, dtype, 0.0, True, seed=51)
+    start = (torch.rand(5003, 1, generator=_gen(52)) < 0.001).to(DEV)
+    got = _grads(ops, q, k, v, g, state, start, do, dfinal)
+    refs, bounds = decay_bounds((q, k, v, g, state, start), dict(do=do, dfinal=dfinal), dtype)
+    for name, x, r, b in zip(("o", "final", "dq", "dk", "dv", "dstate"), got, refs, bounds):
+        assert_close(x, r, b, name)
+
+
+@pytest.mark.parametrize("dtype", ALL, ids=str)
 def test_many_envs(ops, dtype):
     q, k, v, g, state, start, do, dfinal = _case(5, 700, 3, 32, 32, dtype, 0.2, True, seed=8)
     got = _grads(ops, q, k, v, g, state, start, do, dfinal)
@@ -197,16 +208,74 @@ def test_a_step_does_not_see_a_later_one(ops, dtype):
         assert torch.isnan(got[i][at].float()).any()
 
 
-def test_decays_at_their_ends(ops):
-    """no decay at all, at once (-inf), and one so strong that its powers underflow"""
-    q, k, v, _, state, start, do, dfinal = _case(50, 2, 3, 16, 16, torch.float32, 0.05, True, seed=4)
-    g = torch.tensor([0.0, float("-inf"), -60.0], device=DEV)
-    got = _grads(ops, q, k, v, g, state, start, do, dfinal)
-    refs, bounds = decay_bounds((q, k, v, g, state, start), dict(do=do, dfinal=dfinal), torch.float32)
-    for x, r, b in zip(got, refs, bounds):
-        assert_close(x, r, b + 1e-30)
-    only = 16 ** -0.5 * (q[:, :, 1] * k[:, :, 1]).sum(-1, keepdim=True) * v[:, :, 1]  # a head that forgets at once sees its own token
-    assert torch.allclose(got[0][:, :, 1], only, rtol=1e-4, atol=1e-5)
+@pytest.mark.parametrize("dtype", ALL, ids=str)
+def test_decays_at_their_ends(ops, dtype):
+    """no decay at all, at once (-inf), and some so strong that their powers underflow"""
+    q, k, v, _, state, start, do, dfinal = _case(50, 2, 4, 16, 16, dtype, 0.05, True, seed=4)
+    g = torch.tensor([0.0, float("-inf"), -60.0, -9.0], device=DEV)
+    for scale in (None, 1e-4, 30.0):  # (float16 results below its smallest number are zero: half of it is allowed beside the bound)
+        got = _grads(ops, q, k, v, g, state, start, do, dfinal, scale=scale)
+        refs, bounds = decay_bounds((q, k, v, g, state, start), dict(do=do, dfinal=dfinal, scale=scale), dtype)
+        for i, (x, r, b) in enumerate(zip(got, refs, bounds)):
+            assert_close(x, r, b + (2.0 ** -25 if dtype == torch.float16 and x.dtype == dtype else 1e-30), (scale, i))
+        # a head that forgets at once sees its own token
+        own = (16 ** -0.5 if scale is None else scale) * (q[:, :, 1].double() * k[:, :, 1].double()).sum(-1, keepdim=True) * v[:, :, 1].double()
+        assert_close(got[0][:, :, 1], own.cpu(), bounds[0][:, :, 1] + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_small_and_large_values(ops, dtype):
+    """16-bit values far from one: products leave float16's range inside, and the state is still as exact as float32's"""
+    q, k, v, g, state, start, do, dfinal = _case(70, 2, 2, 32, 48, dtype, 0.04, True, seed=31)
+    for a, b, c, d in ((300, 200, 1e-3, 1e-4), (1e-3, 1e-4, 1000, 100), (1e-4, 3000, 3, 1e-4)):
+        args = [(x.float() * f).to(dtype) for x, f in ((q, a), (k, b), (v, c))]
+        dd = (do.float() * d).to(dtype)
+        got = _grads(ops, *args, g, state, start, dd, dfinal)
+        refs, bounds = decay_bounds((*args, g, state, start), dict(do=dd, dfinal=dfinal), dtype)
+        for i, (x, r, e) in enumerate(zip(got, refs, bounds)):
+            most = float(torch.finfo(dtype).max)
+            fits = r.abs() < most * 0.99
+            e = torch.where(fits, e + (2.0 ** -25 if dtype == torch.float16 and x.dtype == dtype else 0), torch.full_like(e, float("inf")))
+            assert_close(torch.where(fits.to(DEV), x, torch.zeros_like(x)), torch.where(fits, r, torch.zeros_like(r)), e, (a, b, c, d, i))
+
+
+def test_an_infinity_leaves_the_others_their_precision(ops):
+    """float16 values are scaled by their largest inside: one that is infinite does not count, or its neighbours would overflow"""
+    dtype, col = torch.float16, 5
+    q, k, v, g, state, _, do, dfinal = _case(75, 2, 2, 32, 48, dtype, 0.0, True, seed=41)
+    other = [j for j in range(48) if j != col]
+
+    def check(q, k, v, state, spoil, o_at, columns):
+        refs, bounds = decay_bounds((q, k, v, g, state), {}, dtype)
+        x, index = spoil
+        x[index] = float("inf")
+        with torch.no_grad():
+            o, final = ops.decay_attention(q, k, v, g, state)
+        assert float(refs[0].abs().max()) < 6e4  # a float16 each
+        assert_close(o[o_at][..., columns], refs[0][o_at][..., columns], bounds[0][o_at][..., columns] + 2.0 ** -25, "o")
+        if columns is other:
+            assert_close(final[..., other], refs[1][..., other], bounds[1][..., other], "state")
+
+    values = v * 1000
+    check(q, k, values, state, (values, (20, 0, 0, col)), slice(None), other)  # one column's token
+    big = q * 1000
+    check(big, k * 1000, v * 3e-4, state * 1e-3, (big, (60, 0, 0, 3)), slice(0, 60), list(range(48)))  # a later query
+    before = state * 1e6
+    check(q * 1e-4, k, v, before, (before, (0, 0, 2, col)), slice(None), other)  # one element remembered
+
+
+def test_a_step_in_place_is_known_to_autograd(ops):
+    """a gradient that still needs the state that a step overwrote is refused, not computed from another state"""
+    q, k, v, g, state, _, do, _ = _case(3, 2, 2, 16, 16, torch.float32, 0.0, True, seed=42)
+    q.requires_grad_()
+    o, _ = ops.decay_attention(q, k, v, g, state)
+    with torch.no_grad():
+        ops.decay_attention_step(q[0], k[0], v[0], g, state, state_out=state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.backward(do)
+    out = torch.empty_like(state, requires_grad=True)
+    with pytest.raises(ValueError, match="no gradient"):
+        ops.decay_attention_step(k[0], k[0], v[0], g, state, state_out=out)
 
 
 def test_missing_gradients_and_scale(ops):
@@ -444,6 +513,32 @@ def test_captured_rollout_step_and_training_step(ops):
         assert all(torch.equal(a, c) for a, c in zip(out, want)) and all(torch.equal(a, c) for a, c in zip(out3, want))
         y2, eager = ops.decay_attention_step(q[0], k[0], v[0], g, eager, start[0])
         assert torch.equal(y, y2) and torch.equal(memory, eager)
+        torch.cuda.synchronize()
+
+
+def test_captured_odd_widths_and_a_long_axis(ops):
+    """two captured passes that need copies of their inputs and the axis cut up, each with its own workspace, replayed in turn"""
+    cases = [_case(steps, 1, 2, 17, 33, torch.float16, 0.01, True, seed=steps) for steps in (700, 1500)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for c in cases:
+            _grads(ops, *c)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in cases], []
+    for graph, c in zip(graphs, cases):
+        with torch.cuda.graph(graph):
+            outs.append(_grads(ops, *c))
+    for i in range(3):
+        for c in cases:
+            for t in c[:3]:
+                t.copy_(torch.randn(t.shape, generator=_gen(60 + i)).to(t.dtype))
+        torch.cuda.synchronize()
+        for graph in graphs:
+            graph.replay()
+        for out, c in zip(outs, cases):
+            assert all(torch.equal(a, b) for a, b in zip(out, _grads(ops, *c)))
         torch.cuda.synchronize()
 
 

@@ -96,6 +96,9 @@ def test_library_refuses_bad_sizes_without_a_gpu(built):
     assert L.urgym_ops_decay(ctypes.byref(s), None, None, None, None) == -1 and b"200" in L.urgym_ops_last_error()
     s = _native.Seq(0, 2, 4, 4, 0, 1)
     assert L.urgym_ops_decay(ctypes.byref(s), None, None, None, None) == -1
+    s = _native.Seq(0, 8, 4, 4, 3, 1 << 20)  # more heads than a launch has room for
+    assert L.urgym_ops_decay(ctypes.byref(s), None, None, None, None) == -1 and b"too large" in L.urgym_ops_last_error()
+    assert L.urgym_ops_decay_workspace(ctypes.byref(s)) == -1
     s = _native.Seq(0, 2, 4, 4, 3, 1)
     assert L.urgym_ops_decay(ctypes.byref(s), None, None, None, None) == -1 and b"needed" in L.urgym_ops_last_error()
     assert L.urgym_ops_decay_step(0, 1, 1, 4, 4, *[None, 0, 0] * 3, None, None, 0, 1.0, None, None, None, None) == -1

@@ -52,13 +52,15 @@ def decay_attention(q, k, v, log_decay, state=None, start=None, scale=None):
         S_t = exp(log_decay) S_{t-1} + k_t v_t^T   (S_{t-1} = 0 where start_t),      o_t = scale S_t^T q_t
 
     q, k: [steps, envs, heads, dk], v: [steps, envs, heads, dv], all float32, bfloat16 or float16, of any strides (slices of one
-    projection, heads expanded from one); dk, dv up to 128.  log_decay: float32 [heads], a constant, 0 or less in use (-inf
-    forgets at once).  state: float32 [envs, heads, dk, dv], what the envs remember from before (None: nothing).
-    start: bool or uint8 [steps, envs], set where a new episode begins -- the step's token does not see what came before it,
-    not even an infinity or NaN.  scale: 1 / sqrt(dk) if None.
+    projection, heads expanded from one); dk, dv up to 128, envs * heads up to 4194304.  log_decay: float32 [heads], a
+    constant, 0 or less (-inf forgets at once; what a greater one gives is not defined).  state: float32
+    [envs, heads, dk, dv], what the envs remember from before (None: nothing).  start: bool or uint8 [steps, envs], set where
+    a new episode begins -- the step's token does not see what came before it, not even an infinity or NaN.  scale:
+    1 / sqrt(dk) if None.
     Returns (o [steps, envs, heads, dv] of q's dtype, the state after the last step).  Products are summed in float32 and
     the state stays in float32; 16-bit inputs meet scores and the carried state rounded to their own type inside the products
-    for o and the gradients.  Differentiable in q, k, v and state; backward computes all three of dq, dk, dv."""
+    for o and the gradients.  What an infinity reaches comes out as infinity or NaN.  Differentiable in q, k, v and state;
+    backward computes all three of dq, dk, dv."""
     return (_ext or _c()).decay_attention(q, k, v, log_decay, state, start, scale)
 
 

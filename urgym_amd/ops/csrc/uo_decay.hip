@@ -237,11 +237,26 @@ __device__ __forceinline__ float wave_max(float x) {
     return fmaxf(fmaxf(lane(0), lane(16)), fmaxf(lane(32), lane(48)));
 }
 
-// 2^-e for a wave-wide largest magnitude in [2^e, 2^(e+1)), and 2^e; 1 for infinities and NaN.  fp16 operands are brought to about
-// one by it: scores and states leave fp16's range long before the outputs do.
+// The largest finite magnitude of the wave's values: `each` hands a lane's to its argument.  (An infinity that one token or column
+// holds must not set the unit of the others; a second look is taken only where there is one.)
+template <class Each>
+__device__ __forceinline__ float largest(Each each) {
+    float most = 0.f;
+    each([&](float x) { most = fmaxf(most, fabsf(x)); });
+    most = wave_max(most);
+    if (most == INFINITY) {
+        most = 0.f;
+        each([&](float x) { most = fabsf(x) < INFINITY ? fmaxf(most, fabsf(x)) : most; });
+        most = wave_max(most);
+    }
+    return most;
+}
+
+// 2^-e for a wave-wide largest magnitude in [2^e, 2^(e+1)), and 2^e; 1 for zero.  fp16 operands are brought to about one by it:
+// scores and states leave fp16's range long before the outputs do.
 __device__ __forceinline__ void unit(float most, float* down, float* up) {
     unsigned e = __float_as_uint(most) & 0x7f800000u;
-    if (e == 0x7f800000u || e < 0x01000000u) e = 0x3f800000u;
+    e = e < 0x01000000u ? 0x3f800000u : e < 0x7e800000u ? e : 0x7e800000u;  // (2^-126 is the smallest normal number)
     *up = __uint_as_float(e);
     *down = __uint_as_float(0x7f000000u - e);
 }
@@ -532,20 +547,22 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
                     for (int e = 0; e < FE; e++) p[it][e] = e / 4 * 16 + e % 4 + 4 * g >= from[it] ? p[it][e] : 0.f;
             float p_down = 1.f, s_down = 1.f, s_up = 1.f;
             if constexpr (F16) {
-                float most = 0.f;
+                auto scores = [&](auto to) {
 #pragma unroll
-                for (int it = 0; it < NB; it++)
+                    for (int it = 0; it < NB; it++)
 #pragma unroll
-                    for (int e = 0; e < FE; e++) most = fmaxf(most, fabsf(p[it][e]));
-                unit(wave_max(most), &p_down, &p_up);
-                most = 0.f;
+                        for (int e = 0; e < FE; e++) to(p[it][e]);
+                };
+                auto state = [&](auto to) {
 #pragma unroll
-                for (int u = 0; u < VA; u++)
+                    for (int u = 0; u < VA; u++)
 #pragma unroll
-                    for (int v = 0; v < VB; v++)
+                        for (int v = 0; v < VB; v++)
 #pragma unroll
-                        for (int r = 0; r < 4; r++) most = fmaxf(most, fabsf(S[u][v][r]));
-                unit(wave_max(most), &s_down, &s_up);
+                            for (int r = 0; r < 4; r++) to(S[u][v][r]);
+                };
+                unit(largest(scores), &p_down, &p_up);
+                unit(largest(state), &s_down, &s_up);
             }
 
             // o, transposed: the carried state's part, weighted by token, then the chunk's own.  Scores and state are rounded to T
@@ -587,16 +604,17 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         // the state: c weighted by its decay to the chunk's end.  In 16 bits the weighted value goes in as two parts of T (to 2^-16 in
         // bf16: enough for o, less than its own rounding), and in bf16 as three where the state itself is an answer, in float32
         // (forward, 500 x 1024 x 4 heads of 64: 261 us with two, 265 with three).  S is touched only where the unit has become small, or, in
-        // fp16, where it does not bring this chunk's c into 2^6 .. 2^15, where both parts have their bits.
+        // fp16, where it does not bring this chunk's weighted c into 2^6 .. 2^15, where both parts have their bits.
         float keep = n_tok < CH ? power(lg, n_tok) : whole, unit_new = s_unit * keep;
         bool off = unit_new < 1.f / 65536 || inside;
         if constexpr (F16) {
-            float most = 0.f, down, up;
+            auto tokens = [&](auto to) {
 #pragma unroll
-            for (int v = 0; v < VB; v++)
+                for (int v = 0; v < VB; v++)
 #pragma unroll
-                for (int e = 0; e < FE; e++) most = fmaxf(most, fabsf((float)fct[v][e]));
-            most = wave_max(most);
+                    for (int e = 0; e < FE; e++) to((float)fct[v][e]);
+            };
+            float down, up, most = largest(tokens) * (fabsf(w.sb) * power(lg, 1 - w.e0));  // times the largest weight
             unit(most, &down, &up);
             off = off || !(most < unit_new * 32768.f) || (most < unit_new * 64.f && most > 0.f);
             unit_new = off ? up * (1.f / 4096) : unit_new;
@@ -933,7 +951,7 @@ static int seq_check(const char* what, int dtype, int64_t steps, int64_t envs, i
     if (dk < 1 || dk > URGYM_OPS_MAX_HEAD_DIM || dv < 1 || dv > URGYM_OPS_MAX_HEAD_DIM)
         return uo_fail("%s: dk %d and dv %d must be 1 .. %d", what, dk, dv, URGYM_OPS_MAX_HEAD_DIM);
     if (steps < 1 || envs < 1 || heads < 1) return uo_fail("%s: steps %lld, envs %lld, heads %d", what, (long long)steps, (long long)envs, heads);
-    if (envs > (1 << 24) || (int64_t)heads * envs > (1 << 24) || steps > (1 << 30))
+    if (envs > URGYM_OPS_MAX_HEADS || (int64_t)heads * envs > URGYM_OPS_MAX_HEADS || steps > (1 << 30))
         return uo_fail("%s: steps %lld, envs %lld, heads %d is too large", what, (long long)steps, (long long)envs, heads);
     return 0;
 }

@@ -263,11 +263,13 @@ static std::tuple<Tensor, Tensor> decay_attention_step(const Tensor& q, const Te
         int64_t apart = (const char*)out.const_data_ptr() - (const char*)state.const_data_ptr();
         TORCH_CHECK_VALUE(apart == 0 || std::abs(apart) >= 4 * state.numel(), "state_out overlaps state without being it");
     }
-    TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad() || state.requires_grad()),
+    TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad() || state.requires_grad() ||
+                                                        (out.defined() && out.requires_grad())),
                       "decay_attention_step has no gradient: call it under torch.no_grad(), or decay_attention for training");
     need_gpu(q);
     at::DeviceGuard guard(q.device());
-    if (!out.defined()) out = at::empty_like(state);
+    if (out.defined()) out.unsafeGetTensorImpl()->bump_version();  // a graph that has saved it must not use what it becomes
+    else out = at::empty_like(state);
     Tensor o = at::empty(v.sizes(), q.options()), a = rows(q), b = rows(k), c = rows(v), g = log_decay.contiguous();
     if (shape[0])
         done(urgym_ops_decay_step(code(q.scalar_type()), shape[0], (int)shape[1], (int)shape[2], (int)shape[3], a.const_data_ptr(), a.stride(0), a.stride(1),
