@@ -412,6 +412,16 @@ def test_layer_norm(ops, shape, affine, dtype):
             assert torch.equal(ops.layer_norm(x, w, b), y)
 
 
+def test_layer_norm_many_wide_rows(ops):
+    """rows that no workgroup holds at once, more of them than workgroups"""
+    x = (torch.randn(700, 8195, generator=_gen(71)) + 0.5).to(DEV).requires_grad_()
+    dy, w = torch.randn(700, 8195, generator=_gen(72)).to(DEV), torch.full((8195,), 1.25, device=DEV, requires_grad=True)
+    y = ops.layer_norm(x, w)
+    refs, bounds = norm_bounds(x.detach(), w.detach(), None, 1e-5, dy)
+    for name, a, r, e in zip(("y", "dx", "dw"), (y, *torch.autograd.grad(y, (x, w), dy)), refs, bounds):
+        assert_close(a, r, e, name)
+
+
 def test_layer_norm_strides_and_partial_gradients(ops):
     x = torch.randn(6, 5, 24, generator=_gen(0)).to(DEV)
     w, b = torch.randn(24, generator=_gen(1)).to(DEV).requires_grad_(), torch.randn(24, generator=_gen(2)).to(DEV).requires_grad_()

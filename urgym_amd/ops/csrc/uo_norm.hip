@@ -227,38 +227,40 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_back(int64_t rows, i
     }
 }
 
-// Rows that no group holds (more than 4096 vectors, or 8192 odd elements): one workgroup a row, the row read again for each pass.
+// Rows that no group holds (more than 4096 vectors, or 8192 odd elements): a workgroup a row at a time, the row read again for each pass.
 template <typename T>
-__global__ __launch_bounds__(1024) void k_norm_wide(int64_t width, const T* x, int64_t xs, const void* w, const void* b, int wdtype,
+__global__ __launch_bounds__(1024) void k_norm_wide(int64_t rows, int64_t width, const T* x, int64_t xs, const void* w, const void* b, int wdtype,
                                                     float eps, T* y, float* mean, float* rstd) {
     __shared__ float lds[2][16];
-    int64_t row = blockIdx.x;
-    const T* xr = x + row * xs;
-    float s = 0.f, q = 0.f;
-    for (int64_t i = threadIdx.x; i < width; i += 1024) s += (float)xr[i];
-    float mu = group_sum<1024>(s, lds[0]) / (float)width;
-    for (int64_t i = threadIdx.x; i < width; i += 1024) q += ((float)xr[i] - mu) * ((float)xr[i] - mu);
-    float r = 1.0f / sqrtf(group_sum<1024>(q, lds[1]) / (float)width + eps);
-    for (int64_t i = threadIdx.x; i < width; i += 1024)
-        y[row * width + i] = (T)(((float)xr[i] - mu) * r * norm_param(w, wdtype, i, 1.f) + norm_param(b, wdtype, i, 0.f));
-    if (mean && threadIdx.x == 0) mean[row] = mu, rstd[row] = r;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T* xr = x + row * xs;
+        float s = 0.f, q = 0.f;
+        for (int64_t i = threadIdx.x; i < width; i += 1024) s += (float)xr[i];
+        float mu = group_sum<1024>(s, lds[0]) / (float)width;
+        for (int64_t i = threadIdx.x; i < width; i += 1024) q += ((float)xr[i] - mu) * ((float)xr[i] - mu);
+        float r = 1.0f / sqrtf(group_sum<1024>(q, lds[1]) / (float)width + eps);
+        for (int64_t i = threadIdx.x; i < width; i += 1024)
+            y[row * width + i] = (T)(((float)xr[i] - mu) * r * norm_param(w, wdtype, i, 1.f) + norm_param(b, wdtype, i, 0.f));
+        if (mean && threadIdx.x == 0) mean[row] = mu, rstd[row] = r;
+    }
 }
 
 template <typename T>
-__global__ __launch_bounds__(1024) void k_norm_wide_dx(int64_t width, const T* dy, int64_t ds, const T* x, int64_t xs, const void* w,
-                                                       int wdtype, const float* mean, const float* rstd, T* dx) {
+__global__ __launch_bounds__(1024) void k_norm_wide_dx(int64_t rows, int64_t width, const T* dy, int64_t ds, const T* x, int64_t xs,
+                                                       const void* w, int wdtype, const float* mean, const float* rstd, T* dx) {
     __shared__ float lds[2][16];
-    int64_t row = blockIdx.x;
-    const T *xr = x + row * xs, *dr = dy + row * ds;
-    float mu = mean[row], r = rstd[row], sg = 0.f, sh = 0.f;
-    for (int64_t i = threadIdx.x; i < width; i += 1024) {
-        float g = (float)dr[i] * norm_param(w, wdtype, i, 1.f);
-        sg += g, sh += g * (((float)xr[i] - mu) * r);
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T *xr = x + row * xs, *dr = dy + row * ds;
+        float mu = mean[row], r = rstd[row], sg = 0.f, sh = 0.f;
+        for (int64_t i = threadIdx.x; i < width; i += 1024) {
+            float g = (float)dr[i] * norm_param(w, wdtype, i, 1.f);
+            sg += g, sh += g * (((float)xr[i] - mu) * r);
+        }
+        sg = group_sum<1024>(sg, lds[0]) / (float)width;
+        sh = group_sum<1024>(sh, lds[1]) / (float)width;
+        for (int64_t i = threadIdx.x; i < width; i += 1024)
+            dx[row * width + i] = (T)(r * ((float)dr[i] * norm_param(w, wdtype, i, 1.f) - sg - ((float)xr[i] - mu) * r * sh));
     }
-    sg = group_sum<1024>(sg, lds[0]) / (float)width;
-    sh = group_sum<1024>(sh, lds[1]) / (float)width;
-    for (int64_t i = threadIdx.x; i < width; i += 1024)
-        dx[row * width + i] = (T)(r * ((float)dr[i] * norm_param(w, wdtype, i, 1.f) - sg - ((float)xr[i] - mu) * r * sh));
 }
 
 template <typename T>
@@ -325,7 +327,7 @@ static bool norm_group(int64_t units, F&& f) {
     return false;
 }
 
-// workgroups of the forward pass: enough to fill the chip, several rows each beyond that
+// workgroups of the forward pass (and of wide rows): enough to fill the chip, several rows each beyond that
 static unsigned norm_blocks(int64_t rows, int per_block, int block) {
     int64_t n = (rows + per_block - 1) / per_block, most = 256 * 2048 / block;
     return (unsigned)(n < most ? n : most);
@@ -388,7 +390,7 @@ static int norm_fwd(int64_t rows, int64_t width, const void* x, int64_t xs, cons
         done = norm_group<true>(width / V, NormForward<T, V>{rows, width, x, xs, w, b, wdtype, eps, y, mean, rstd, st});
     else
         done = norm_group<false>(width, NormForward<T, 1>{rows, width, x, xs, w, b, wdtype, eps, y, mean, rstd, st});
-    if (!done) k_norm_wide<T><<<(unsigned)rows, 1024, 0, st>>>(width, (const T*)x, xs, w, b, wdtype, eps, (T*)y, mean, rstd);
+    if (!done) k_norm_wide<T><<<norm_blocks(rows, 1, 1024), 1024, 0, st>>>(rows, width, (const T*)x, xs, w, b, wdtype, eps, (T*)y, mean, rstd);
     return uo_launched("urgym_ops_layer_norm");
 }
 
@@ -404,7 +406,7 @@ static int norm_bwd(int64_t rows, int64_t width, const void* dy, int64_t ds, con
             done = norm_group<true>(width / V, NormBackward<T, V>{rows, width, dy, ds, x, xs, w, wdtype, mean, rstd, dx, ws, st});
         else
             done = norm_group<false>(width, NormBackward<T, 1>{rows, width, dy, ds, x, xs, w, wdtype, mean, rstd, dx, ws, st});
-        if (!done && dx) k_norm_wide_dx<T><<<(unsigned)rows, 1024, 0, st>>>(width, (const T*)dy, ds, (const T*)x, xs, w, wdtype, mean, rstd, (T*)dx);
+        if (!done && dx) k_norm_wide_dx<T><<<norm_blocks(rows, 1, 1024), 1024, 0, st>>>(rows, width, (const T*)dy, ds, (const T*)x, xs, w, wdtype, mean, rstd, (T*)dx);
         if (!done && ws)
             k_norm_wide_dw<T><<<dim3((unsigned)parts, (unsigned)((width + 63) / 64)), 64, 0, st>>>(rows, width, (const T*)dy, ds, (const T*)x, xs, mean, rstd, ws);
     }

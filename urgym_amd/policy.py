@@ -67,7 +67,7 @@ class MemoryPolicy(torch.nn.Module):
 
     def initial_state(self, envs):
         """one state per block: nothing remembered"""
-        return [torch.zeros(envs, self.heads, self.head_dim, self.head_dim, device=self.log_decay.device) for _ in self.blocks]
+        return [torch.zeros(envs, self.heads, self.head_dim, self.head_dim, dtype=torch.float32, device=self.log_decay.device) for _ in self.blocks]
 
     def _run(self, obs, attend):
         x = self.embed(obs.to(self.embed.weight.dtype))
