@@ -62,7 +62,7 @@ struct Sweep {
 struct Sweeps {
     Sweep w[3];
     unsigned count, slices, segs, heads;  // sweeps in this launch, waves for each of them and segment of the axis, segments
-    int columns;                          // of C that a wave holds
+    int tile, columns;                    // tile width of a and b, columns of C that a wave holds
     unsigned items;                       // envs * heads * count * slices * segs waves
     int seg_len;                          // steps in a segment (the last may be shorter)
     int64_t steps;
@@ -809,22 +809,22 @@ static void launch_tile(const Sweeps& s, hipStream_t st) {
 
 template <typename T>
 static void launch(const Sweeps& s, hipStream_t st) {
-    if (s.w[0].da <= 32) launch_tile<T, Tile<T, 32, 2>>(s, st);
-    else if (s.w[0].da <= 64 && s.columns == 64) launch_tile<T, Tile<T, 64, 4>>(s, st);
-    else if (s.w[0].da <= 64) launch_tile<T, Tile<T, 64, 2>>(s, st);
+    if (s.tile == 32) launch_tile<T, Tile<T, 32, 2>>(s, st);
+    else if (s.tile == 64 && s.columns == 64) launch_tile<T, Tile<T, 64, 4>>(s, st);
+    else if (s.tile == 64) launch_tile<T, Tile<T, 64, 2>>(s, st);
     else launch_tile<T, Tile<T, 128, 2>>(s, st);
 }
 
 static int tile(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
-// The launch of `count` sweeps whose a and b fall into one tile width.  With fewer waves than fill the chip twice over (one a SIMD is
+// The launch of `count` sweeps, of the widest one's tile.  With fewer waves than fill the chip twice over (one a SIMD is
 // half of that) the axis is cut into segments, at least 64 steps each: their states are computed first, then joined.
 static Sweeps plan(const urgym_ops_seq* q, const Sweep* w, int count) {
     Sweeps s = {};
     s.count = count, s.heads = q->heads, s.steps = q->steps, s.log_decay = q->log_decay;
-    int db = 0;
-    for (int i = 0; i < count; i++) s.w[i] = w[i], db = w[i].db > db ? w[i].db : db;
-    s.columns = columns_of(tile(w[0].da), db, q->envs * q->heads * count * ((db + 63) / 64)), s.slices = (db + s.columns - 1) / s.columns;
+    int db = 0, da = 0;
+    for (int i = 0; i < count; i++) s.w[i] = w[i], da = w[i].da > da ? w[i].da : da, db = w[i].db > db ? w[i].db : db;
+    s.tile = tile(da), s.columns = columns_of(s.tile, db, q->envs * q->heads * count * ((db + 63) / 64)), s.slices = (db + s.columns - 1) / s.columns;
     s.items = (unsigned)(q->envs * q->heads) * s.count * s.slices;
     int64_t segs = s.items >= FILL ? 1 : 2 * FILL / s.items, most = q->steps / 64;
     segs = segs < most ? segs : most;
@@ -838,10 +838,10 @@ static Sweeps plan(const urgym_ops_seq* q, const Sweep* w, int count) {
 }
 
 // in floats, whole vectors
-static int64_t workspace(const Sweeps& s) { return s.segs > 1 ? ((int64_t)s.items * (tile(s.w[0].da) * s.columns + 1) + 3) / 4 * 4 : 0; }
+static int64_t workspace(const Sweeps& s) { return s.segs > 1 ? ((int64_t)s.items * (s.tile * s.columns + 1) + 3) / 4 * 4 : 0; }
 
 static void launch(const urgym_ops_seq* q, Sweeps s, float* ws, hipStream_t st) {
-    s.ws = ws, s.left = ws + (int64_t)s.items * tile(s.w[0].da) * s.columns;
+    s.ws = ws, s.left = ws + (int64_t)s.items * s.tile * s.columns;
     if (q->dtype == URGYM_OPS_F32) launch<float>(s, st);
     else if (q->dtype == URGYM_OPS_BF16) launch<bf16>(s, st);
     else launch<f16>(s, st);
@@ -1005,7 +1005,7 @@ static Rows readable(const urgym_ops_seq* s, Rows r, int d, float* ws, int64_t* 
 }
 
 // Everything one direction enqueues, and its workspace: copies of what cannot be read as it is, then the launches of o's sweep, or
-// of those of dk, dq and dv, which read the same rows and share a launch where their tiles agree.
+// of those of dk, dq and dv, which read the same rows and share a launch where their tiles agree or may.
 struct Work {
     Packs packs;
     Sweeps sweeps[2];
@@ -1027,7 +1027,10 @@ static Work work(const urgym_ops_seq* s, const Rows* g, float* ws) {
         Rows d = readable(s, *g, s->dv, ws, &w.floats, &w.packs);
         Sweep b[3] = {backward(s, v, d, q, none, s->dv, s->dk, true, nullptr), forward(s, d, v, k, none, s->dv, s->dk, true),
                       backward(s, k, q, d, none, s->dk, s->dv, false, nullptr)};
-        if (tile(s->dk) == tile(s->dv)) w.sweeps[w.count++] = plan(s, b, 3);
+        // Tiles of 32 and 64 in 16 bits share the wider one where waves are few and launches count (24 and 40 wide heads, float16, 333 x
+        // 185: 61 -> 49 us, 333 x 370: 91 -> 69, but 333 x 740: 95 -> 106); others never gain (64 and 128, bf16, 333 x 370: 93 -> 125).
+        bool few = s->dtype != URGYM_OPS_F32 && s->dk <= 64 && s->dv <= 64 && s->envs * s->heads < FILL / 2;
+        if (tile(s->dk) == tile(s->dv) || few) w.sweeps[w.count++] = plan(s, b, 3);
         else w.sweeps[w.count++] = plan(s, b, 2), w.sweeps[w.count++] = plan(s, b + 2, 1);
     }
     w.ws = ws + w.floats;
