@@ -818,7 +818,9 @@ static void launch(const Sweeps& s, hipStream_t st) {
 static int tile(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 // The launch of `count` sweeps, of the widest one's tile.  With fewer waves than fill the chip twice over (one a SIMD is
-// half of that) the axis is cut into segments, at least 64 steps each: their states are computed first, then joined.
+// half of that) the axis is cut into segments, at least 32 steps each: their states are computed first, then joined.  That costs a
+// pass, so fewer than 3 segments or 128 steps stay whole (forward, 4 heads of 32, 500 steps, float32: 26 us with 64 steps or more a
+// segment, 21 with 32; 200 heads, 130 steps, bf16: 16.8 us in 2 segments, 13.5 whole).
 static Sweeps plan(const urgym_ops_seq* q, const Sweep* w, int count) {
     Sweeps s = {};
     s.count = count, s.heads = q->heads, s.steps = q->steps, s.log_decay = q->log_decay;
@@ -826,10 +828,10 @@ static Sweeps plan(const urgym_ops_seq* q, const Sweep* w, int count) {
     for (int i = 0; i < count; i++) s.w[i] = w[i], da = w[i].da > da ? w[i].da : da, db = w[i].db > db ? w[i].db : db;
     s.tile = tile(da), s.columns = columns_of(s.tile, db, q->envs * q->heads * count * ((db + 63) / 64)), s.slices = (db + s.columns - 1) / s.columns;
     s.items = (unsigned)(q->envs * q->heads) * s.count * s.slices;
-    int64_t segs = s.items >= FILL ? 1 : 2 * FILL / s.items, most = q->steps / 64;
+    int64_t segs = s.items >= FILL ? 1 : 2 * FILL / s.items, most = q->steps / 32;
     segs = segs < most ? segs : most;
     segs = segs < MAX_SEGS ? segs : MAX_SEGS;
-    if (segs < 2) segs = 1;
+    if (segs < 3 || most < 4) segs = 1;
     int64_t len = (q->steps + segs - 1) / segs;
     len = (len + 31) / 32 * 32;
     s.segs = (unsigned)((q->steps + len - 1) / len), s.seg_len = (int)len;
