@@ -63,11 +63,12 @@ int64_t urgym_ops_decay_workspace(const urgym_ops_seq* s);
 int64_t urgym_ops_decay_backward_workspace(const urgym_ops_seq* s, const void* d_out, const int64_t d_out_stride[3]);
 
 /* S_t = exp(log_decay) S_{t-1} + k_t v_t^T (S_{t-1} = 0 where start_t), o_t = scale S_t^T q_t.
- * o [steps, envs, heads, dv], state_out float32 [envs, heads, dk, dv] (S of the last step), both contiguous. */
+ * log_decay: 0 or less.  o [steps, envs, heads, dv], state_out float32 [envs, heads, dk, dv] (S of the last step), both
+ * contiguous and apart from the inputs. */
 int urgym_ops_decay(const urgym_ops_seq* s, void* o, float* state_out, float* workspace, void* stream);
 
 /* The gradients of urgym_ops_decay: from d_out (strides d_out_stride, as q's) and d_state_out (NULL: zero, contiguous) to
- * dq, dk, dv (contiguous, of dtype; all three wanted or NULL each) and d_state (NULL: not wanted). */
+ * dq, dk, dv (contiguous, of dtype, all three needed) and d_state (NULL: not wanted), apart from the inputs. */
 int urgym_ops_decay_backward(const urgym_ops_seq* s, const void* d_out, const int64_t d_out_stride[3],
                              const float* d_state_out, void* dq, void* dk, void* dv, float* d_state, float* workspace,
                              void* stream);
