@@ -100,6 +100,20 @@ def test_many_envs(ops, dtype):
         assert_close(x, r, b)
 
 
+@pytest.mark.parametrize("dtype", ALL, ids=str)
+@pytest.mark.parametrize("envs", [7, 120, 173, 300])
+def test_many_heads_of_two_widths(ops, envs, dtype):
+    """keys and values of different widths, few heads (one launch for all gradients) to many (two), 32 and 64 columns a wave.
+    (The bounds count a rounding as half a step relative to the value.  Below 2^-14 float16's steps no longer shrink with the
+    value: they are 2^-24 all the way to zero, so the rounding of an answer there is off by up to 2^-25, whatever its size.)"""
+    for steps, dk, dv in ((35, 20, 40), (6, 64, 24)):
+        q, k, v, g, state, start, do, dfinal = _case(steps, envs, 3, dk, dv, dtype, 0.1, True, seed=envs)
+        got = _grads(ops, q, k, v, g, state, start, do, dfinal)
+        refs, bounds = decay_bounds((q, k, v, g, state, start), dict(do=do, dfinal=dfinal), dtype)
+        for i, (x, r, b) in enumerate(zip(got, refs, bounds)):
+            assert_close(x, r, b + (2.0 ** -25 if x.dtype == torch.float16 else 0), (steps, i))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
 def test_strides(ops, dtype):
     """slices of one projection, env-major storage, heads expanded from one, uint8 starts of any stride, odd offsets"""

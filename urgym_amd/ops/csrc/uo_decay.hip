@@ -27,6 +27,12 @@
 //   * o is computed transposed, so that a lane holds neighbouring columns of one token, which it stores as a vector;
 //   * 16-bit operands that contract the tokens are transposed on their way out of LDS.
 // LDS rows are swizzled in blocks of 16 bytes, so that both kinds of reads spread over the banks.
+//
+// Heads of up to 64 are bound by memory: 500 x 1024 x 4 heads of 64 in bf16 take 260 us forward (1.05 GB: 4.0 TB/s; the same loads and
+// stores without the products 209 to 235) and 510 to 560 backward (dq runs against the time of dk and dv, so its inputs are read
+// again: 7 reads and 3 writes, 2.62 GB, 4.7 to 5.1 TB/s), and fewer waves a CU change nothing until they are 8.  Heads of 128 are bound
+// by the chunk's latency: LDS leaves 8 waves a CU (500 x 4096 heads: 685 us for 2.1 GB; 64 columns a wave are slower yet, 45.6 against
+// 41.8 us at 200 x 512).  So are few heads: a wave alone on its SIMD takes 4 to 5 us a chunk, hence the segments.
 #include "uo_common.h"
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -744,8 +750,8 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
 }
 
 // The states that the segments begin with, from what each adds: begin_0 = what enters, begin_{s+1} = left_s begin_s + added_s.
-// A workgroup takes 32 float4s of one wave's accumulators; its 8 rows of
-// threads take a run of PER segments each, all of whose loads are in flight at once, then hand on through LDS.
+// A workgroup takes 32 float4s of one wave's accumulators; its 8 rows of threads take a run of PER segments each, all of whose loads
+// are in flight at once, then hand on through LDS (8 heads of 64, 128 segments: 9 us for 34 MB in and out, most of it latency).
 constexpr int RUNS = 8, MAX_SEGS = RUNS * 16;
 
 template <class L, int PER>
@@ -851,7 +857,7 @@ static void launch(const urgym_ops_seq* q, Sweeps s, float* ws, hipStream_t st) 
 
 // One token: W waves of a workgroup take one (env, head).  LPR lanes hold a row of the state, E elements each (neighbours, as one
 // vector, or LPR apart where dv is odd), and 64 / LPR rows are under way at once in each wave, 8 times over: the state's bytes, in and
-// out, are the whole cost.  The columns' sums over the rows are joined across lanes, then through LDS across the waves.
+// out, are the whole cost (4096 x 4 heads of 64: 99 us, 5.4 TB/s).  The columns' sums over the rows are joined across lanes, then through LDS across the waves.
 template <typename T, int E, bool VEC, int LPR>
 __global__ __launch_bounds__(256) void k_step(int heads, int dk, int dv, Rows q, Rows k, Rows v, const float* log_decay,
                                               const uint8_t* start, int64_t start_sn, float scale, const float* s_in,
