@@ -24,7 +24,8 @@ extern "C" const char* urgym_ops_last_error(void) { return uo_message; }
 // A row is held by a group of G threads, K vectors of V elements each (V elements = 16 bytes, or 1 where a width, stride or
 // address is odd), so x and dy are read once from memory; the statistics are the mean, then the centred second moment of the
 // values in registers (E[x^2] - mean^2 would cancel).  Groups walk over the rows with the weights kept in registers and the next row
-// already on its way.  Both directions are bound by memory: 2 (forward) and 3 (backward) row passes, 512000 x 256 in bf16 in 97 us (5.4
+// already on its way, as it lies in memory (converted on arrival instead, its wait would come at once: 20000 x 999 in f16 40 us backward, 84
+// so).  Both directions are bound by memory: 2 (forward) and 3 (backward) row passes, 512000 x 256 in bf16 in 97 us (5.4
 // TB/s) and 160 us (4.9 TB/s).
 template <typename T, int V>
 struct Vec {
@@ -36,12 +37,21 @@ struct Vec<T, 1> {
 };
 
 template <typename T, int V>
-__device__ __forceinline__ void norm_load(float* to, const T* p) {
-    typename Vec<T, V>::type v = *(const typename Vec<T, V>::type*)p;
+__device__ __forceinline__ typename Vec<T, V>::type norm_ask(const T* p) {
+    return *(const typename Vec<T, V>::type*)p;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void norm_take(float* to, typename Vec<T, V>::type v) {
     if constexpr (V == 1) to[0] = (float)v;
     else
 #pragma unroll
         for (int e = 0; e < V; e++) to[e] = (float)v[e];
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void norm_load(float* to, const T* p) {
+    norm_take<T, V>(to, norm_ask<T, V>(p));
 }
 
 template <typename T, int V>
@@ -96,17 +106,18 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm(int64_t rows, int64_
     __shared__ float lds[2][G > UO_WAVE ? G / UO_WAVE : 1];
     int t = threadIdx.x % G;
     int64_t row = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G, stride = (int64_t)gridDim.x * (BLOCK / G);
-    float wv[K][V], bv[K][V], next[K][V];
+    float wv[K][V], bv[K][V];
+    typename Vec<T, V>::type next[K];
     const float inv = 1.f / (float)width;
     bool have[K];
 #pragma unroll
     for (int k = 0; k < K; k++) {
         int64_t i = (int64_t)(k * G + t) * V;
-        have[k] = i < width;
+        have[k] = i < width, next[k] = (T)0.f;
 #pragma unroll
-        for (int e = 0; e < V; e++) wv[k][e] = bv[k][e] = next[k][e] = 0.f;
+        for (int e = 0; e < V; e++) wv[k][e] = bv[k][e] = 0.f;
         if (have[k]) {
-            if (row < rows) norm_load<T, V>(next[k], x + row * xs + i);
+            if (row < rows) next[k] = norm_ask<T, V>(x + row * xs + i);
             norm_params<T, V>(wv[k], w, wdtype, i, 1.f);
             norm_params<T, V>(bv[k], b, wdtype, i, 0.f);
         }
@@ -115,9 +126,10 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm(int64_t rows, int64_
         float v[K][V], s = 0.f;
 #pragma unroll
         for (int k = 0; k < K; k++) {
+            norm_take<T, V>(v[k], next[k]);
 #pragma unroll
-            for (int e = 0; e < V; e++) v[k][e] = next[k][e], s += v[k][e];
-            if (have[k] && row + stride < rows) norm_load<T, V>(next[k], x + (row + stride) * xs + (int64_t)(k * G + t) * V);
+            for (int e = 0; e < V; e++) s += v[k][e];
+            if (have[k] && row + stride < rows) next[k] = norm_ask<T, V>(x + (row + stride) * xs + (int64_t)(k * G + t) * V);
         }
         float mu = group_sum<G>(s, lds[0]) / (float)width, q = 0.f;
 #pragma unroll
@@ -149,39 +161,43 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_back(int64_t rows, i
     __shared__ float cols[G > UO_WAVE ? 1 : 2 * 4 * G * K * V];
     int t = threadIdx.x % G;
     int64_t row = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G, stride = (int64_t)gridDim.x * (BLOCK / G);
-    float wv[K][V], dw[K][V], db[K][V], nx[K][V], nd[K][V], n_mu = 0.f, n_r = 0.f;
+    float wv[K][V], dw[K][V], db[K][V], n_mu = 0.f, n_r = 0.f;
+    typename Vec<T, V>::type nx[K], nd[K];
     const float inv = 1.f / (float)width;
     bool have[K];
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-        int64_t i = (int64_t)(k * G + t) * V;
-        have[k] = i < width;
-#pragma unroll
-        for (int e = 0; e < V; e++) wv[k][e] = dw[k][e] = db[k][e] = nx[k][e] = nd[k][e] = 0.f;
-        if (have[k]) {
-            if (row < rows) norm_load<T, V>(nx[k], x + row * xs + i), norm_load<T, V>(nd[k], dy + row * ds + i);
-            norm_params<T, V>(wv[k], w, wdtype, i, 1.f);
-        }
-    }
-    if (row < rows) n_mu = mean[row], n_r = rstd[row];
-    for (; row < rows; row += stride) {
-        float h[K][V], d[K][V], mu = n_mu, r = n_r, sg = 0.f, sh = 0.f;
-        bool more = row + stride < rows;
+    auto fetch = [&](int64_t r) {
 #pragma unroll
         for (int k = 0; k < K; k++) {
+            int64_t i = (int64_t)(k * G + t) * V;
+            if (have[k]) nx[k] = norm_ask<T, V>(x + r * xs + i), nd[k] = norm_ask<T, V>(dy + r * ds + i);
+        }
+        n_mu = mean[r], n_r = rstd[r];
+    };
+#pragma unroll
+    for (int k = 0; k < K; k++) have[k] = (int64_t)(k * G + t) * V < width, nx[k] = nd[k] = (T)0.f;
+    if (row < rows) fetch(row);
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+#pragma unroll
+        for (int e = 0; e < V; e++) wv[k][e] = dw[k][e] = db[k][e] = 0.f;
+        if (have[k]) norm_params<T, V>(wv[k], w, wdtype, (int64_t)(k * G + t) * V, 1.f);
+    }
+    for (; row < rows; row += stride) {
+        float h[K][V], d[K][V], mu = n_mu, r = n_r, sg = 0.f, sh = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            norm_take<T, V>(h[k], nx[k]), norm_take<T, V>(d[k], nd[k]);
 #pragma unroll
             for (int e = 0; e < V; e++) {
-                h[k][e] = (nx[k][e] - mu) * r, d[k][e] = nd[k][e];
+                h[k][e] = (h[k][e] - mu) * r;
                 if (have[k]) {
                     dw[k][e] += d[k][e] * h[k][e], db[k][e] += d[k][e];
                     float gr = d[k][e] * wv[k][e];
                     sg += gr, sh += gr * h[k][e];
                 }
             }
-            int64_t i = (int64_t)(k * G + t) * V;
-            if (have[k] && more) norm_load<T, V>(nx[k], x + (row + stride) * xs + i), norm_load<T, V>(nd[k], dy + (row + stride) * ds + i);
         }
-        if (more) n_mu = mean[row + stride], n_r = rstd[row + stride];
+        if (row + stride < rows) fetch(row + stride);
         if (!dx) continue;
         sg = group_sum<G>(sg, lds[0]) * inv;
         sh = group_sum<G>(sh, lds[1]) * inv;
