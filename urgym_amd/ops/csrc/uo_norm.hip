@@ -26,7 +26,7 @@ extern "C" const char* urgym_ops_last_error(void) { return uo_message; }
 // values in registers (E[x^2] - mean^2 would cancel).  Groups walk over the rows with the weights kept in registers and the next row
 // already on its way, as it lies in memory (converted on arrival instead, its wait would come at once: 20000 x 999 in f16 40 us backward, 84
 // so).  Both directions are bound by memory: 2 (forward) and 3 (backward) row passes, 512000 x 256 in bf16 in 97 us (5.4
-// TB/s) and 160 us (4.9 TB/s).
+// TB/s) and 155 us (5.1 TB/s).
 template <typename T, int V>
 struct Vec {
     typedef T type __attribute__((ext_vector_type(V)));
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(64) void k_norm_wide_dw(int64_t rows, int64_t width
 }
 
 // the workgroups' sums added up in a fixed order: 32 columns by 32 runs of parts to a workgroup, the runs then through LDS (latency:
-// 5 us for 256 columns of 1024 parts; 7 us, 2.9 TB/s, for 5000 of 512)
+// 5 us for 256 columns of 768 parts, 4 us, 2.4 TB/s, for 5000 of 256)
 __global__ __launch_bounds__(1024) void k_norm_dw_sum(int64_t width, int64_t parts, const float* ws, void* dw, void* db, int wdtype) {
     __shared__ float lds[32][33];
     void* to = blockIdx.y ? db : dw;
@@ -351,10 +351,13 @@ static unsigned norm_blocks(int64_t rows, int per_block, int block) {
     return (unsigned)(n < most ? n : most);
 }
 
-// Workgroups of the backward pass, each of which leaves a part of the column sums: half of what fills the chip, so that parts (two
-// floats a column) stay small beside the rows.
+// Workgroups of the backward pass, each of which leaves a part of the column sums (two floats a column, written and read again):
+// about as many as it takes to have 2 MB on the way.  Backward, f16: 512000 x 256 143 us with 768, 151 with 1024, 155 with 512;
+// 10000 x 2048 30 with 512, 39 with 256, 32 with 768; 4097 x 5000 35.5 with 256, 40.5 with 512; single elements, 20000 x 999: 30 with
+// 1024, 40 with 512.
 static int64_t norm_parts(int64_t rows, int64_t width) {
-    int64_t rows_a_time = width <= 512 ? 8 : 1, most = width <= 512 ? 1024 : 512, n = (rows + rows_a_time - 1) / rows_a_time;
+    int64_t rows_a_time = width <= 512 ? 8 : 1, n = (rows + rows_a_time - 1) / rows_a_time;
+    int64_t most = width <= 512 ? 768 : width % 8 && width <= 2048 ? 1024 : width < 4096 ? 512 : 256;
     return n < most ? n : most;
 }
 
