@@ -58,9 +58,9 @@ def decay_attention(q, k, v, log_decay, state=None, start=None, scale=None):
     a new episode begins -- the step's token does not see what came before it, not even an infinity or NaN.  scale:
     1 / sqrt(dk) if None.
     Returns (o [steps, envs, heads, dv] of q's dtype, the state after the last step).  Products are summed in float32 and
-    the state stays in float32; 16-bit inputs meet scores and the carried state rounded to their own type inside the products
-    for o and the gradients.  What an infinity reaches comes out as infinity or NaN.  Differentiable in q, k, v and state;
-    backward computes all three of dq, dk, dv."""
+    the state stays in float32; over more than 32 steps, 16-bit inputs meet the carried state rounded to their own type
+    inside the products for o and the gradients.  What an infinity reaches comes out as infinity or NaN.
+    Differentiable in q, k, v and state; backward computes all three of dq, dk, dv."""
     return (_ext or _c()).decay_attention(q, k, v, log_decay, state, start, scale)
 
 

@@ -29,9 +29,9 @@
 // LDS rows are swizzled in blocks of 16 bytes, so that both kinds of reads spread over the banks.
 //
 // Heads of up to 64 are bound by memory: 500 x 1024 x 4 heads of 64 in bf16 take 260 us forward (1.05 GB: 4.0 TB/s; the same loads and
-// stores without the products 209 to 235) and 510 to 560 backward (dq runs against the time of dk and dv, so its inputs are read
-// again: 7 reads and 3 writes, 2.62 GB, 4.7 to 5.1 TB/s), and fewer waves a CU change nothing until they are 8.  Heads of 128 are bound
-// by the chunk's latency: LDS leaves 8 waves a CU (500 x 4096 heads: 685 us for 2.1 GB; 64 columns a wave are slower yet, 45.6 against
+// stores without the products 209 to 235) and 520 to 580 backward (dq runs against the time of dk and dv, so its inputs are read
+// again: 7 reads and 3 writes, 2.62 GB, 4.5 to 5.0 TB/s), and fewer waves a CU change nothing until they are 8.  Heads of 128 are bound
+// by the chunk's latency: LDS leaves 8 waves a CU (500 x 4096 heads: 730 us for 2.1 GB; 64 columns a wave are slower yet, 45.6 against
 // 41.8 us at 200 x 512).  So are few heads: a wave alone on its SIMD takes 4 to 5 us a chunk, hence the segments.
 #include "uo_common.h"
 
@@ -463,6 +463,14 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         rows_of(Int<RC>(), pc, stc, L::C0, db - j0, x, n_tok);
     };
 
+    // element e of y's two parts
+    const bool fine = HALF && all.steps <= CH;
+    auto parts = [&](float y, Frag& hi, Frag& lo, int e) {
+        asm("" : "+v"(y));  // rounded here, for both
+        hi[e] = (T)y;
+        if (HALF) lo[e] = (T)(y - (float)hi[e]);
+    };
+
     // One chunk: the operands from LDS, then (`next`: the next chunk's loads begin) o and the state, then (`done`: they have landed)
     // the stores.  False, and nothing done, where the chunk has to be taken in parts.
     auto compute = [&](int x, int n_tok, bool fresh, unsigned inside, auto next, auto done) {
@@ -571,9 +579,11 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
                 unit(largest(state), &s_down, &s_up);
             }
 
-            // o, transposed: the carried state's part, weighted by token, then the chunk's own.  Scores and state are rounded to T
-            // here: an error of half a step of T in each product, as large as that of the output's own rounding.
-            Frag fp[NB];
+            // o, transposed: the carried state's part, weighted by token, then the chunk's own.  In 16 bits the scores go in as two parts
+            // of T, and so does the state where the whole axis is one chunk, for then it is what the caller handed in and often most
+            // of o.  Elsewhere it is rounded to T here: half a step of T in each product, as the output's own rounding, whose error
+            // grows by at most 1.4.  (500 x 4096 heads of 64, bf16, backward: 516 us with one part each, 529 so, 582 with two of each.)
+            Frag fp[NB], fp_lo[NB];
             float by_token[NB];
 #pragma unroll
             for (int it = 0; it < NB; it++) by_token[it] = carry[it] * s_unit;
@@ -586,23 +596,32 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
 #pragma unroll
             for (int it = 0; it < NB; it++)
 #pragma unroll
-                for (int e = 0; e < FE; e++) fp[it][e] = (T)(F16 ? p[it][e] * p_down : p[it][e]);
+                for (int e = 0; e < FE; e++) parts(F16 ? p[it][e] * p_down : p[it][e], fp[it], fp_lo[it], e);
 #pragma unroll
             for (int v = 0; v < VB; v++) {
-                Frag fs[NF];
+                f4 acc[NB];
 #pragma unroll
-                for (int i = 0; i < L::DA / 4; i++) {
-                    int u = HALF ? i / 4 : i % VA, r = HALF ? i % 4 : i / VA;
-                    fs[i / FE][i % FE] = (T)(F16 ? S[u][v][r] * s_down : S[u][v][r]);
+                for (int it = 0; it < NB; it++) acc[it] = (f4)0.f;
+#pragma unroll
+                for (int f = 0; f < NF; f++) {
+                    Frag fs, fs_lo;
+#pragma unroll
+                    for (int e = 0; e < FE; e++) {
+                        int i = f * FE + e, u = HALF ? i / 4 : i % VA, r = HALF ? i % 4 : i / VA;
+                        parts(F16 ? S[u][v][r] * s_down : S[u][v][r], fs, fs_lo, e);
+                    }
+#pragma unroll
+                    for (int it = 0; it < NB; it++) acc[it] = dot(acc[it], fs, fa[it][f]);
+                    if (fine)
+#pragma unroll
+                        for (int it = 0; it < NB; it++) acc[it] = dot(acc[it], fs_lo, fa[it][f]);
                 }
 #pragma unroll
                 for (int it = 0; it < NB; it++) {
-                    f4 acc = (f4)0.f;
-#pragma unroll
-                    for (int f = 0; f < NF; f++) acc = dot(acc, fs[f], fa[it][f]);
-                    acc *= F16 ? by_token[it] * (s_up * p_down) : by_token[it];
-                    if (inside && from[it]) acc = (f4)0.f;
-                    O[it][v] = dot(acc, fct[v], fp[it]);
+                    acc[it] *= F16 ? by_token[it] * (s_up * p_down) : by_token[it];
+                    if (inside && from[it]) acc[it] = (f4)0.f;
+                    O[it][v] = dot(acc[it], fct[v], fp[it]);
+                    if (HALF) O[it][v] = dot(O[it][v], fct[v], fp_lo[it]);
                 }
             }
         }
