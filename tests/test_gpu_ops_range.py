@@ -1,0 +1,116 @@
+"""The decay attention over inputs whose magnitudes differ widely between columns, tokens and dimensions -- against the definition in
+64 bits (tests/ops_reference.py)."""
+import pytest
+import torch
+
+from ops_reference import assert_close, decay_bounds
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+ALL = [torch.float32, torch.bfloat16, torch.float16]
+NAMES = ("o", "final", "dq", "dk", "dv", "dstate")
+
+
+@pytest.fixture(scope="module")
+def ops(built):
+    from urgym_amd import ops
+    return ops
+
+
+def _inputs(steps, envs, heads, dk, dv, seed):
+    """float32 on the CPU: q, k, v, log_decay, state, do, dfinal"""
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    decay = torch.log1p(-1.0 / torch.logspace(0.5, 6, heads, base=2.0)) if heads > 1 else torch.tensor([-0.1])
+    return dict(q=r(steps, envs, heads, dk), k=r(steps, envs, heads, dk), v=r(steps, envs, heads, dv), g=decay,
+                state=3 * r(envs, heads, dk, dv), do=r(steps, envs, heads, dv), dfinal=r(envs, heads, dk, dv))
+
+
+def _on_gpu(x, dtype):
+    return {n: (t.to(dtype) if n in ("q", "k", "v", "do") else t).to(DEV) for n, t in x.items()}
+
+
+def _run(ops, x, start=None, **kw):
+    leaves = [x[n].detach().requires_grad_() for n in ("q", "k", "v", "state")]
+    o, final = ops.decay_attention(*leaves[:3], x["g"], leaves[3], start, **kw)
+    return [o, final, *torch.autograd.grad((o, final), leaves, (x["do"], x["dfinal"]))]
+
+
+def _reference(x, start=None, bounds=decay_bounds):
+    return bounds((x["q"], x["k"], x["v"], x["g"], x["state"], start), dict(do=x["do"], dfinal=x["dfinal"]), x["q"].dtype)
+
+
+def _compare(got, refs, bounds, dtype, what):
+    """(float16 answers below 2^-14 are rounded by up to 2^-25 whatever their size; those beyond its largest number do not count)"""
+    for name, y, r, b in zip(NAMES, got, refs, bounds):
+        if y.dtype == torch.float16:
+            fits = r.abs() < 0.99 * torch.finfo(dtype).max
+            y, r, b = torch.where(fits.to(DEV), y, torch.zeros_like(y)), torch.where(fits, r, torch.zeros_like(r)), b + 2.0 ** -25
+        assert_close(y, r, b, (what, name))
+
+
+def _column(x, ratio):
+    x["v"] *= 2.0 ** -7
+    x["v"][..., 5] *= ratio
+
+
+def _state_column(x, ratio):
+    x["state"][..., 5] *= ratio
+    x["q"] *= 2.0 ** -2
+
+
+def _state_column_that_no_gradient_reads(x, ratio):
+    x["state"][..., 5] *= ratio
+    x["v"][..., 5] *= 2.0 ** 8
+    x["do"][..., 5] = 0
+    x["dfinal"][..., 5] = 0
+
+
+def _query_tokens(x, ratio):
+    x["q"] *= 2.0 ** -6
+    x["q"][20::25] *= ratio
+
+
+def _gradient_steps(x, ratio):
+    x["do"] *= 2.0 ** -6
+    x["do"][20::25] *= ratio
+
+
+def _key_dimension_that_no_query_reads(x, ratio):
+    x["k"] *= 2.0 ** -6
+    x["k"][..., 3] *= ratio
+    x["state"][..., 3, :] *= ratio
+    x["q"][..., 3] = 0
+
+
+def _keys_large_where_values_are_small(x, ratio):
+    x["k"][10::3] *= ratio ** 0.5
+    x["v"][10::3] *= ratio ** -0.5
+    x["q"] *= 2.0 ** -2
+
+
+@pytest.mark.parametrize("dtype", ALL, ids=str)
+@pytest.mark.parametrize("change,ratio", [(_column, 12), (_column, 16), (_column, 20), (_state_column, 12), (_state_column, 20), (_state_column, 40),
+                                          (_state_column_that_no_gradient_reads, 30), (_query_tokens, 14), (_query_tokens, 20),
+                                          (_gradient_steps, 14), (_gradient_steps, 20), (_key_dimension_that_no_query_reads, 20),
+                                          (_keys_large_where_values_are_small, 20)], ids=lambda c: c.__name__[1:] if callable(c) else str(c))
+def test_magnitudes_that_differ(ops, change, ratio, dtype):
+    """a column, token or dimension 2^ratio times the others: those keep their precision"""
+    x = _inputs(70, 2, 2, 32, 48, 7)
+    change(x, 2.0 ** ratio)
+    x = _on_gpu(x, dtype)
+    assert all(torch.isfinite(t).all() for t in x.values())
+    for starts in (None, (0, 23, 41, 43)):
+        start = None
+        if starts:
+            start = torch.zeros(70, 2, dtype=torch.bool, device=DEV)
+            start[list(starts)] = True
+        _compare(_run(ops, x, start), *_reference(x, start), dtype, (change.__name__, ratio, starts))
+
+
+@pytest.mark.parametrize("dtype", ALL, ids=str)
+@pytest.mark.parametrize("scale", [1e-3, 40.0, -40.0])
+def test_scales_far_from_one(ops, scale, dtype):
+    x = _on_gpu(_inputs(45, 2, 2, 24, 40, 9), dtype)
+    refs, bounds = decay_bounds((x["q"], x["k"], x["v"], x["g"], x["state"]), dict(do=x["do"], dfinal=x["dfinal"], scale=scale), dtype)
+    _compare(_run(ops, x, scale=scale), refs, bounds, dtype, scale)

@@ -61,7 +61,8 @@ struct Sweep {
     float* s_out;       // NULL: not wanted
     const uint8_t* s_drop;  // backward: the flags [envs] (stride start_sn) that cut the state's gradient
     int s_i, s_j;
-    float sa, sb, in_mul, out_mul;
+    bool answer;  // the state is an answer, or may be: tokens enter it in three parts, whether s_out is wanted or not
+    float sa, sb;
     int e0;
 };
 
@@ -85,6 +86,9 @@ template <typename T>
 struct Kind {
     static constexpr bool HALF = sizeof(T) == 2, F16 = __is_same(T, f16);
 };
+// the numbers of bfloat16 (float32's range) that hold an element of T exactly: its operands' parts in products with what is computed
+template <typename T>
+constexpr int PARTS = Kind<T>::F16 ? 2 : 1;
 template <typename T>
 struct FragOf {
     typedef f4 type;
@@ -96,6 +100,15 @@ struct FragOf<bf16> {
 template <>
 struct FragOf<f16> {
     typedef f16x8 type;
+};
+// operands of products with what is computed
+template <typename T>
+struct PartOf {
+    typedef bf16x8 type;
+};
+template <>
+struct PartOf<float> {
+    typedef f4 type;
 };
 
 // A wave's tiles in LDS: CH tokens of a and b (DA wide) and of 16 VB columns of c
@@ -128,6 +141,17 @@ __device__ __forceinline__ f4 dot(f4 acc, f16x8 a, f16x8 b) { return __builtin_a
 __device__ __forceinline__ f4 dot(f4 acc, f4 a, f4 b) {
 #pragma unroll
     for (int i = 0; i < 4; i++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc, 0, 0, 0);
+    return acc;
+}
+
+// acc += x y for factors in parts, the largest first, but for products of two parts below what the sums of parts leave out
+template <class P, int X, int Y>
+__device__ __forceinline__ f4 dots(f4 acc, const P (&x)[X], const P (&y)[Y]) {
+    constexpr int MOST = X > Y ? X : Y;
+#pragma unroll
+    for (int i = 0; i < X; i++)
+#pragma unroll
+        for (int j = 0; j < Y && i + j < MOST; j++) acc = dot(acc, x[i], y[j]);
     return acc;
 }
 
@@ -233,43 +257,57 @@ __device__ __forceinline__ void columns(u4* to, const char* tile, int c, int g) 
     }
 }
 
-// the largest of a wave's values, none of them negative
-__device__ __forceinline__ float wave_max(float x) {
-    x = fmaxf(x, uo_dpp<0xB1>(x));   // lane ^ 1
-    x = fmaxf(x, uo_dpp<0x4E>(x));   // lane ^ 2
-    x = fmaxf(x, uo_dpp<0x141>(x));  // the mirror in 8
-    x = fmaxf(x, uo_dpp<0x140>(x));  // the mirror in 16
-    auto lane = [&](int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), i)); };
-    return fmaxf(fmaxf(lane(0), lane(16)), fmaxf(lane(32), lane(48)));
+// N parts of a fragment of float32 numbers, each the rest after those before it, rounded; y becomes what is left.  (The pair is
+// opaque to the compiler, which would convert each of the two by itself as well.)
+template <int N>
+__device__ __forceinline__ void split(f4 (&to)[N], float (&y)[4]) {
+    static_assert(N == 1);
+    to[0] = f4{y[0], y[1], y[2], y[3]};
 }
-
-// The largest finite magnitude of the wave's values: `each` hands a lane's to its argument.  (An infinity that one token or column
-// holds must not set the unit of the others; a second look is taken only where there is one.)
-template <class Each>
-__device__ __forceinline__ float largest(Each each) {
-    float most = 0.f;
-    each([&](float x) { most = fmaxf(most, fabsf(x)); });
-    most = wave_max(most);
-    if (most == INFINITY) {
-        most = 0.f;
-        each([&](float x) { most = fabsf(x) < INFINITY ? fmaxf(most, fabsf(x)) : most; });
-        most = wave_max(most);
+template <int N>
+__device__ __forceinline__ void split(bf16x8 (&to)[N], float (&y)[8]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        u4 pairs;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+            unsigned w = __builtin_bit_cast(unsigned, bf16x2{(bf16)y[e], (bf16)y[e + 1]});
+            asm("" : "+v"(w));
+            y[e] -= __uint_as_float(w << 16), y[e + 1] -= __uint_as_float(w & 0xffff0000u);
+            pairs[e / 2] = w;
+        }
+        to[i] = __builtin_bit_cast(bf16x8, pairs);
     }
-    return most;
 }
 
-// 2^-e for a wave-wide largest magnitude in [2^e, 2^(e+1)), and 2^e; 1 for zero.  fp16 operands are brought to about one by it:
-// scores and states leave fp16's range long before the outputs do.
-__device__ __forceinline__ void unit(float most, float* down, float* up) {
-    unsigned e = __float_as_uint(most) & 0x7f800000u;
-    e = e < 0x01000000u ? 0x3f800000u : e < 0x7e800000u ? e : 0x7e800000u;  // (2^-126 is the smallest normal number)
-    *up = __uint_as_float(e);
-    *down = __uint_as_float(0x7f000000u - e);
+// y, rounded here: a product fused into a subtraction of split() would give that another y
+__device__ __forceinline__ float rounded(float y) {
+    asm("" : "+v"(y));
+    return y;
+}
+
+// The operand x of a product with what is computed, as numbers of bfloat16 whose sum it is: float16 takes two (8 bits and the 3 that
+// are left).  What is computed is rounded to bfloat16's parts, whose range is float32's, never to float16: scores and states leave that
+// range, and no one scale brings columns, tokens and dimensions of very different magnitudes into it.
+__device__ __forceinline__ void parts_of(bf16x8 (&to)[1], bf16x8 x) { to[0] = x; }
+__device__ __forceinline__ void parts_of(f4 (&to)[1], f4 x) { to[0] = x; }
+__device__ __forceinline__ void parts_of(bf16x8 (&to)[2], f16x8 x) {
+    u4 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float y[2], l[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) y[e] = (float)x[2 * i + e], l[e] = y[e] - __uint_as_float(__float_as_uint(y[e]) & 0xffff0000u);
+        hi[i] = __builtin_amdgcn_perm(__float_as_uint(y[1]), __float_as_uint(y[0]), 0x07060302u);  // both upper halves
+        lo[i] = __builtin_amdgcn_perm(__float_as_uint(l[1]), __float_as_uint(l[0]), 0x07060302u);
+    }
+    to[0] = __builtin_bit_cast(bf16x8, hi), to[1] = __builtin_bit_cast(bf16x8, lo);
 }
 
 // element (i, j) of the state that enters the sweep
 __device__ __forceinline__ float entering(const Sweep& w, unsigned nh, int i, int j) {
-    return w.s_in && i < w.da && j < w.db ? w.in_mul * w.s_in[(int64_t)nh * w.da * w.db + i * w.s_i + j * w.s_j] : 0.f;
+    return w.s_in && i < w.da && j < w.db ? w.s_in[(int64_t)nh * w.da * w.db + i * w.s_i + j * w.s_j] : 0.f;
 }
 
 // All of a lane's elements of the state at p, unscaled, or to p: as vectors where its elements are neighbours, the tiles are full and p
@@ -359,8 +397,10 @@ __device__ __forceinline__ f4 joined(f4 x, float left, f4 add) { return left == 
 template <typename T, class L, bool STATE>
 __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
     typedef typename FragOf<T>::type Frag;
+    typedef typename PartOf<T>::type Part;
     constexpr int FE = L::FE, NB = L::NB, CH = L::CH, NF = L::NF, VA = L::VA, VB = L::VB, RA = L::RA, RC = L::RC;
-    constexpr bool HALF = Kind<T>::HALF, F16 = Kind<T>::F16;
+    constexpr bool HALF = Kind<T>::HALF;
+    constexpr int P = PARTS<T>, TWO = HALF ? 2 : 1;
     __shared__ __attribute__((aligned(256))) char lds[L::LDS];
     // workgroups go to the 8 XCDs in turn: each takes a run of items, for neighbours share rows -- the slices, then the sweeps,
     // then the heads of one env -- and their L2
@@ -395,7 +435,7 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
 
     // C = unit * S: a chunk's decay goes into the unit, and into the tokens that enter, instead of into all of S
     f4 S[VA][VB];
-    float s_unit = STATE || all.segs > OWN_JOIN || !w.s_in ? 1.f : w.in_mul;
+    float s_unit = 1.f;
 #pragma unroll
     for (int u = 0; u < VA; u++)
 #pragma unroll
@@ -404,12 +444,11 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
     if (!STATE && all.segs <= OWN_JOIN) {
         for (unsigned before = seg; before; before--) {
             unsigned other = item - before * all.count * all.slices;
-            float left = all.left[other] * s_unit;
+            float left = all.left[other];
 #pragma unroll
             for (int u = 0; u < VA; u++)
 #pragma unroll
                 for (int v = 0; v < VB; v++) S[u][v] = joined(S[u][v], left, *held(all, other, VA * VB, u * VB + v, lane));
-            s_unit = 1.f;
         }
     }
 
@@ -463,14 +502,7 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         rows_of(Int<RC>(), pc, stc, L::C0, db - j0, x, n_tok);
     };
 
-    // element e of y's two parts
-    const bool fine = HALF && all.steps <= CH;
-    auto parts = [&](float y, Frag& hi, Frag& lo, int e) {
-        asm("" : "+v"(y));  // rounded here, for both
-        hi[e] = (T)y;
-        if (HALF) lo[e] = (T)(y - (float)hi[e]);
-    };
-
+    const bool fine = !HALF || all.steps <= CH;
     // One chunk: the operands from LDS, then (`next`: the next chunk's loads begin) o and the state, then (`done`: they have landed)
     // the stores.  False, and nothing done, where the chunk has to be taken in parts.
     auto compute = [&](int x, int n_tok, bool fresh, unsigned inside, auto next, auto done) {
@@ -537,7 +569,6 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         }
 
         f4 O[NB][VB];
-        float p_up = 1.f;
         if constexpr (!STATE) {
             // scores, transposed: row j = 4 g + r, column i = c
             f4 sc[NB][NB];
@@ -559,31 +590,16 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
                 for (int it = 0; it < NB; it++)
 #pragma unroll
                     for (int e = 0; e < FE; e++) p[it][e] = e / 4 * 16 + e % 4 + 4 * g >= from[it] ? p[it][e] : 0.f;
-            float p_down = 1.f, s_down = 1.f, s_up = 1.f;
-            if constexpr (F16) {
-                auto scores = [&](auto to) {
-#pragma unroll
-                    for (int it = 0; it < NB; it++)
-#pragma unroll
-                        for (int e = 0; e < FE; e++) to(p[it][e]);
-                };
-                auto state = [&](auto to) {
-#pragma unroll
-                    for (int u = 0; u < VA; u++)
-#pragma unroll
-                        for (int v = 0; v < VB; v++)
-#pragma unroll
-                            for (int r = 0; r < 4; r++) to(S[u][v][r]);
-                };
-                unit(largest(scores), &p_down, &p_up);
-                unit(largest(state), &s_down, &s_up);
-            }
 
-            // o, transposed: the carried state's part, weighted by token, then the chunk's own.  In 16 bits the scores go in as two parts
-            // of T, and so does the state where the whole axis is one chunk, for then it is what the caller handed in and often most
-            // of o.  Elsewhere it is rounded to T here: half a step of T in each product, as the output's own rounding, whose error
-            // grows by at most 1.4.  (500 x 4096 heads of 64, bf16, backward: 516 us with one part each, 529 so, 582 with two of each.)
-            Frag fp[NB], fp_lo[NB];
+            // o, transposed: the carried state's part, weighted by token, then the chunk's own.  16-bit operands meet scores and states
+            // as two numbers of bfloat16 (2^-16), but for states met by bfloat16 in axes of several chunks: one number.
+            Part fp[NB][TWO];
+#pragma unroll
+            for (int it = 0; it < NB; it++)
+#pragma unroll
+                for (int e = 0; e < FE; e++) p[it][e] = rounded(p[it][e]);
+#pragma unroll
+            for (int it = 0; it < NB; it++) split(fp[it], p[it]);
             float by_token[NB];
 #pragma unroll
             for (int it = 0; it < NB; it++) by_token[it] = carry[it] * s_unit;
@@ -596,56 +612,45 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
 #pragma unroll
             for (int it = 0; it < NB; it++)
 #pragma unroll
-                for (int e = 0; e < FE; e++) parts(F16 ? p[it][e] * p_down : p[it][e], fp[it], fp_lo[it], e);
+                for (int v = 0; v < VB; v++) O[it][v] = (f4)0.f;
 #pragma unroll
-            for (int v = 0; v < VB; v++) {
-                f4 acc[NB];
+            for (int f = 0; f < NF; f++) {
+                Part pa[NB][P];
 #pragma unroll
-                for (int it = 0; it < NB; it++) acc[it] = (f4)0.f;
+                for (int it = 0; it < NB; it++) parts_of(pa[it], fa[it][f]);
 #pragma unroll
-                for (int f = 0; f < NF; f++) {
-                    Frag fs, fs_lo;
+                for (int v = 0; v < VB; v++) {
+                    Part fs[TWO];
+                    float y[FE];
 #pragma unroll
                     for (int e = 0; e < FE; e++) {
                         int i = f * FE + e, u = HALF ? i / 4 : i % VA, r = HALF ? i % 4 : i / VA;
-                        parts(F16 ? S[u][v][r] * s_down : S[u][v][r], fs, fs_lo, e);
+                        y[e] = S[u][v][r];
                     }
+                    split(fs, y);
 #pragma unroll
-                    for (int it = 0; it < NB; it++) acc[it] = dot(acc[it], fs, fa[it][f]);
-                    if (fine)
-#pragma unroll
-                        for (int it = 0; it < NB; it++) acc[it] = dot(acc[it], fs_lo, fa[it][f]);
+                    for (int it = 0; it < NB; it++) O[it][v] = P == 2 || fine ? dots(O[it][v], fs, pa[it]) : dot(O[it][v], fs[0], pa[it][0]);
                 }
+            }
+#pragma unroll
+            for (int v = 0; v < VB; v++) {
+                Part pc[P];
+                parts_of(pc, fct[v]);
 #pragma unroll
                 for (int it = 0; it < NB; it++) {
-                    acc[it] *= F16 ? by_token[it] * (s_up * p_down) : by_token[it];
-                    if (inside && from[it]) acc[it] = (f4)0.f;
-                    O[it][v] = dot(acc[it], fct[v], fp[it]);
-                    if (HALF) O[it][v] = dot(O[it][v], fct[v], fp_lo[it]);
+                    O[it][v] *= by_token[it];
+                    if (inside && from[it]) O[it][v] = (f4)0.f;
+                    O[it][v] = dots(O[it][v], pc, fp[it]);
                 }
             }
         }
 
-        // the state: c weighted by its decay to the chunk's end.  In 16 bits the weighted value goes in as two parts of T (to 2^-16 in
-        // bf16: enough for o, less than its own rounding), and in bf16 as three where the state itself is an answer, in float32
-        // (forward, 500 x 1024 x 4 heads of 64: 261 us with two, 265 with three).  S is touched only where the unit has become small, or, in
-        // fp16, where it does not bring this chunk's weighted c into 2^6 .. 2^15, where both parts have their bits.
+        // the state: c weighted by its decay to the chunk's end.  In 16 bits the weighted value goes in as two parts (2^-16, enough
+        // for o), and as three where the state itself is an answer, in float32 (forward, 500 x 1024 x 4 heads of 64, bf16: 261 us with
+        // two, 265 with three).  S is touched only where the unit has become small.
         float keep = n_tok < CH ? power(lg, n_tok) : whole, unit_new = s_unit * keep;
-        bool off = unit_new < 1.f / 65536 || inside;
-        if constexpr (F16) {
-            auto tokens = [&](auto to) {
-#pragma unroll
-                for (int v = 0; v < VB; v++)
-#pragma unroll
-                    for (int e = 0; e < FE; e++) to((float)fct[v][e]);
-            };
-            float down, up, most = largest(tokens) * (fabsf(w.sb) * power(lg, 1 - w.e0));  // times the largest weight
-            unit(most, &down, &up);
-            off = off || !(most < unit_new * 32768.f) || (most < unit_new * 64.f && most > 0.f);
-            unit_new = off ? up * (1.f / 4096) : unit_new;
-        } else {
-            unit_new = off ? 1.f : unit_new;
-        }
+        const bool off = unit_new < 1.f / 65536 || inside;
+        unit_new = off ? 1.f : unit_new;
         if (__builtin_amdgcn_readfirstlane(off)) {
             keep *= s_unit * __builtin_amdgcn_rcpf(unit_new);
 #pragma unroll
@@ -661,25 +666,26 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         for (int e = 0; e < FE; e++) by[e] = !inside || e / 4 * 16 + e % 4 + 4 * g >= last ? enter[e] * grow : 0.f;
 #pragma unroll
         for (int v = 0; v < VB; v++) {
-            Frag hi, lo, rest;
+            Part y[TWO], rest[1];
             float z[FE];
 #pragma unroll
-            for (int e = 0; e < FE; e++) {
-                float y = (float)fct[v][e] * by[e];
-                asm("" : "+v"(y));  // y is rounded here: its product fused into one of the conversions would give that another hi
-                hi[e] = (T)y, z[e] = y - (float)hi[e];
-                if (HALF) lo[e] = (T)z[e];
-            }
+            for (int e = 0; e < FE; e++) z[e] = rounded((float)fct[v][e] * by[e]);
+            split(y, z);
 #pragma unroll
             for (int u = 0; u < VA; u++) {
-                S[u][v] = dot(S[u][v], fbt[u], hi);
-                if (HALF) S[u][v] = dot(S[u][v], fbt[u], lo);
+                Part pb[P];
+                parts_of(pb, fbt[u]);
+                S[u][v] = dots(S[u][v], pb, y);
             }
-            if (HALF && !F16 && w.s_out) {
+            if (HALF && w.answer) {
+                split(rest, z);
 #pragma unroll
-                for (int e = 0; e < FE; e++) rest[e] = (T)(z[e] - (float)lo[e]);
-#pragma unroll
-                for (int u = 0; u < VA; u++) S[u][v] = dot(S[u][v], fbt[u], rest);
+                for (int u = 0; u < VA; u++) {
+                    Part pb[P];
+                    parts_of(pb, fbt[u]);
+                    S[u][v] = dot(S[u][v], pb[0], rest[0]);
+                    if (P == 2) S[u][v] = dot(S[u][v], pb[P - 1], y[TWO - 1]);
+                }
             }
         }
         done();
@@ -699,7 +705,7 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
 #pragma unroll
                             for (int i = 0; i < N; i++) {
                                 int v = HALF ? 2 * q + (e + i) / 4 : (e + i) % VB, r = HALF ? (e + i) % 4 : (e + i) / VB;
-                                y.v[i] = (T)(F16 ? O[it][v][r] * p_up : O[it][v][r]);
+                                y.v[i] = (T)O[it][v][r];
                             }
                             if (e + N <= left) {
                                 *(Piece<T, N>*)(to + 32 * q + e) = y;
@@ -765,7 +771,7 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
     }
     if (!w.s_out || seg + 1 < all.segs) return;
     bool drop = w.s_drop && w.s_drop[n * w.start_sn];
-    state_store<L>(S, w.out_mul * s_unit, drop, w, w.s_out + (int64_t)nh * da * db, j0, c, g);
+    state_store<L>(S, s_unit, drop, w, w.s_out + (int64_t)nh * da * db, j0, c, g);
 }
 
 // The states that the segments begin with, from what each adds: begin_0 = what enters, begin_{s+1} = left_s begin_s + added_s.
@@ -1004,19 +1010,18 @@ static Sweep forward(const urgym_ops_seq* s, Rows a, Rows b, Rows c, Rows o, int
     Sweep w = {};
     w.a = a, w.b = b, w.c = c, w.o = o, w.da = da, w.db = db;
     w.start = s->start, w.start_st = s->start_stride[0], w.start_sn = s->start_stride[1], w.first = true;
-    w.s_in = s->state, w.s_i = transposed ? 1 : db, w.s_j = transposed ? da : 1;
-    w.sa = s->scale, w.sb = 1.f, w.in_mul = 1.f, w.out_mul = 1.f, w.e0 = 1;
+    w.s_in = s->state, w.s_i = transposed ? 1 : db, w.s_j = transposed ? da : 1, w.answer = !transposed;
+    w.sa = s->scale, w.sb = 1.f, w.e0 = 1;
     return w;
 }
 
 // dk or dv: against time's order from d_state_out.  Token x of the sweep is step steps - 1 - x, which an episode border cuts from
-// token x - 1 where step steps - x starts one.  A scale above 1 stays outside the state: times a c of float16 it could overflow.
+// token x - 1 where step steps - x starts one.
 static Sweep backward(const urgym_ops_seq* s, Rows a, Rows b, Rows c, Rows o, int da, int db, bool transposed, const float* d_state_out) {
     Sweep w = forward(s, reversed(a, s), reversed(b, s), reversed(c, s), reversed(o, s), da, db, transposed);
     if (s->start) w.start = s->start + s->steps * s->start_stride[0], w.start_st = -s->start_stride[0];
     w.first = false, w.e0 = 0, w.s_in = d_state_out, w.s_drop = s->start;
-    if (s->scale > 1.f || s->scale < -1.f) w.sa = s->scale, w.sb = 1.f, w.in_mul = 1.f / s->scale, w.out_mul = s->scale;
-    else w.sa = 1.f, w.sb = s->scale;
+    w.sa = 1.f, w.sb = s->scale;
     return w;
 }
 
