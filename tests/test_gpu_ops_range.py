@@ -1,9 +1,9 @@
-"""The decay attention over inputs whose magnitudes differ widely between columns, tokens and dimensions -- against the definition in
-64 bits (tests/ops_reference.py)."""
+"""The decay attention over inputs whose magnitudes differ widely between columns, tokens and dimensions, its precision beyond one
+chunk, and what reaches far along a cut axis -- against the definition in 64 bits (tests/ops_reference.py)."""
 import pytest
 import torch
 
-from ops_reference import assert_close, decay_bounds
+from ops_reference import U32, assert_close, decay_bounds, decay_reference, half_step
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -114,3 +114,24 @@ def test_scales_far_from_one(ops, scale, dtype):
     x = _on_gpu(_inputs(45, 2, 2, 24, 40, 9), dtype)
     refs, bounds = decay_bounds((x["q"], x["k"], x["v"], x["g"], x["state"]), dict(do=x["do"], dfinal=x["dfinal"], scale=scale), dtype)
     _compare(_run(ops, x, scale=scale), refs, bounds, dtype, scale)
+
+
+def _rounded_once(args, kw, dtype):
+    """float32 throughout (n32 M as in decay_bounds) but for the inputs' and outputs' own type, and 16-bit types' products: their
+    factors are held to 2^-16 (two bfloat16 numbers, half a step each) and products of two second parts are left out (2^-8 2^-8, with
+    float16's operands 2^-8 2^-7), once where a token enters the state and once where the state is read, or in scores and values."""
+    mags, refs = decay_reference(*args, **kw, magnitude=True), decay_reference(*args, **kw)
+    steps, g = args[0].shape[0], float(args[3].double().abs().max())
+    n32 = (2 * (steps + 256) + steps * (4 + g)) * U32
+    inner = {torch.float32: 0.0, torch.bfloat16: 2 * 2.0 ** -16, torch.float16: 2 * (2.0 ** -16 + 2.0 ** -15)}[dtype]
+    return refs, [(n32 + (2 * half_step(dtype) ** 2 if i in (1, 5) and dtype == torch.float16 else 0 if i in (1, 5) else inner)) * m
+                  + (U32 if i in (1, 5) else half_step(dtype)) * r.abs() + 1e-30 for i, (m, r) in enumerate(zip(mags, refs))]
+
+
+@pytest.mark.parametrize("dtype", ALL, ids=str)
+@pytest.mark.parametrize("steps,dk,dv", [(33, 1, 40), (33, 40, 1), (90, 1, 1), (70, 2, 64), (70, 64, 2), (40, 128, 1), (40, 1, 128)])
+def test_answers_are_rounded_once(ops, steps, dk, dv, dtype):
+    """the state carried from chunk to chunk is not rounded on its way into an answer.  (Heads of one key or value dimension: an answer is
+    one product of the state, so a second rounding shows.)"""
+    x = _on_gpu(_inputs(steps, 3, 2, dk, dv, steps + dk), dtype)
+    _compare(_run(ops, x), *_reference(x, bounds=_rounded_once), dtype, (steps, dk, dv))
