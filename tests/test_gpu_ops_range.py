@@ -135,3 +135,32 @@ def test_answers_are_rounded_once(ops, steps, dk, dv, dtype):
     one product of the state, so a second rounding shows.)"""
     x = _on_gpu(_inputs(steps, 3, 2, dk, dv, steps + dk), dtype)
     _compare(_run(ops, x), *_reference(x, bounds=_rounded_once), dtype, (steps, dk, dv))
+
+
+@pytest.mark.parametrize("dtype", ALL, ids=str)
+def test_what_a_long_axis_keeps_of_an_infinity_or_nan(ops, dtype):
+    """no episode starts, so a NaN reaches every later answer however small its weight has become: also where the axis is cut into
+    pieces, and a piece's decay is nothing in float32"""
+    steps, at = 3000, 40
+    x = _on_gpu(_inputs(steps, 1, 2, 32, 24, 11), dtype)
+    x["g"] = torch.tensor([-6.0, float("-inf")], device=DEV)  # exp(-6 * 32) is zero in float32
+    for name, value in (("k", float("nan")), ("v", float("inf"))):
+        y = dict(x, **{name: x[name].clone()})
+        y[name][at, ..., 3] = value
+        with torch.no_grad():
+            o, final = ops.decay_attention(y["q"], y["k"], y["v"], y["g"], y["state"])
+        columns = slice(None) if name == "k" else slice(3, 4)
+        assert not torch.isfinite(o[at:, ..., columns].float()).any() and torch.isfinite(o[:at].float()).all()
+        assert not torch.isfinite(final[:, :, 3] if name == "k" else final[..., 3]).any()
+    y = dict(x, do=x["do"].clone())
+    y["do"][steps - at, ..., 3] = float("nan")
+    got = _run(ops, y)
+    assert torch.isnan(got[3][:steps - at].float()).all() and torch.isnan(got[4][:steps - at, ..., 3].float()).all()
+    assert torch.isfinite(got[3][steps - at + 1:].float()).all()
+    start = torch.zeros(steps, 1, dtype=torch.bool, device=DEV)
+    start[1500] = True  # from here on nothing is seen of it
+    y = dict(x, k=x["k"].clone())
+    y["k"][at] = float("nan")
+    with torch.no_grad():
+        o, final = ops.decay_attention(y["q"], y["k"], y["v"], y["g"], y["state"], start)
+    assert torch.isnan(o[at:1500].float()).all() and torch.isfinite(o[1500:].float()).all() and torch.isfinite(final).all()

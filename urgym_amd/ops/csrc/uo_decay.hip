@@ -75,12 +75,13 @@ struct Sweeps {
     int64_t steps;
     const float* log_decay;
     // segs > 1: for each wave what its segment adds to the state, or (after k_join) the state it begins with, as the wave's
-    // accumulators lie in its registers; and the factor that it leaves of the state before it.  Up to OWN_JOIN segments, each
+    // accumulators lie in its registers; and the factor that it leaves of the state before it, CUT where an episode starts in it.  Up to OWN_JOIN segments, each
     // wave joins what lies before its own.
     float *ws, *left;
 };
 
 constexpr unsigned OWN_JOIN = 8;
+constexpr float CUT = -1.f;  // (not zero: a decay may underflow to that, and then still hands on an infinity or NaN)
 
 template <typename T>
 struct Kind {
@@ -388,8 +389,8 @@ __device__ __forceinline__ f4* held(const Sweeps& all, unsigned item, int tiles,
     return (f4*)all.ws + ((int64_t)item * tiles + tile) * UO_WAVE + lane;
 }
 
-// the state after a segment that leaves `left` of x and adds `add` (selected where it leaves nothing: nothing passes a start)
-__device__ __forceinline__ f4 joined(f4 x, float left, f4 add) { return left == 0.f ? add : x * left + add; }
+// the state after a segment that leaves `left` of x and adds `add` (selected: nothing passes a start)
+__device__ __forceinline__ f4 joined(f4 x, float left, f4 add) { return left == CUT ? add : x * left + add; }
 
 // STATE: only what the segment adds to the state (no a, no o); segments after it need that before they can begin.
 // Two waves a SIMD at least, that is 256 registers at most: then matrix instructions accumulate in ordinary registers, where C is
@@ -766,7 +767,7 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         for (int u = 0; u < VA; u++)
 #pragma unroll
             for (int v = 0; v < VB; v++) *held(all, item, VA * VB, u * VB + v, lane) = S[u][v] * s_unit;
-        if (lane == 0) all.left[item] = any ? 0.f : power(lg, steps);
+        if (lane == 0) all.left[item] = any ? CUT : power(lg, steps);
         return;
     }
     if (!w.s_out || seg + 1 < all.segs) return;
@@ -805,7 +806,7 @@ __global__ __launch_bounds__(256) void k_join(Sweeps all) {
     f4 x = (f4)0.f;
     float l = 1.f;
 #pragma unroll
-    for (int i = 0; i < PER; i++) x = joined(x, left[i], add[i]), l *= left[i];
+    for (int i = 0; i < PER; i++) x = joined(x, left[i], add[i]), l = l == CUT || left[i] == CUT ? CUT : l * left[i];
     sums[run][threadIdx.x % 32] = x;
     if (threadIdx.x % 32 == 0) lefts[run] = l;
     __syncthreads();
