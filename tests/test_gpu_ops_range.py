@@ -164,3 +164,18 @@ def test_what_a_long_axis_keeps_of_an_infinity_or_nan(ops, dtype):
     with torch.no_grad():
         o, final = ops.decay_attention(y["q"], y["k"], y["v"], y["g"], y["state"], start)
     assert torch.isnan(o[at:1500].float()).all() and torch.isfinite(o[1500:].float()).all() and torch.isfinite(final).all()
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "state"])
+def test_no_steps_still_have_gradients(ops, which):
+    """an empty rollout: nothing answered, the state as it was, and a backward pass"""
+    x = _on_gpu(_inputs(3, 2, 2, 8, 12, 12), torch.float32)
+    x = {n: (t[:0] if n in ("q", "k", "v", "do") else t) for n, t in x.items()}
+    leaf = x[which] = x[which].detach().requires_grad_()
+    o, final = ops.decay_attention(x["q"], x["k"], x["v"], x["g"], x["state"])
+    assert o.shape == (0, 2, 2, 12) and torch.equal(final, x["state"])
+    ((o * x["do"]).sum() + (final * x["dfinal"]).sum()).backward()
+    assert torch.equal(leaf.grad, x["dfinal"] if which == "state" else torch.zeros_like(leaf))
+    with torch.no_grad():
+        o, final = ops.decay_attention(x["q"], x["k"], x["v"], x["g"])
+    assert o.shape == (0, 2, 2, 12) and not final.any() and final.shape == x["state"].shape

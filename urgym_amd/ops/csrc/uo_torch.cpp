@@ -188,7 +188,10 @@ static std::tuple<Tensor, Tensor> decay_forward(const Tensor& q, const Tensor& k
                                                 const Tensor& start, double scale) {
     at::DeviceGuard guard(q.device());
     Tensor o = at::empty(v.sizes(), q.options());
-    Tensor final = at::empty({q.size(1), q.size(2), q.size(3), v.size(3)}, q.options().dtype(at::kFloat));
+    const int64_t shape[4] = {q.size(1), q.size(2), q.size(3), v.size(3)};
+    if (q.size(0) == 0)  // no step: nothing is answered and nothing forgotten
+        return {o, state.defined() ? state.clone() : at::zeros(shape, q.options().dtype(at::kFloat))};
+    Tensor final = at::empty(shape, q.options().dtype(at::kFloat));
     if (q.size(1)) {
         urgym_ops_seq s = sequence(q, k, v, log_decay, state, start, scale);
         Tensor ws = workspace(urgym_ops_decay_workspace(&s), q);
@@ -215,8 +218,11 @@ struct DecayAttention : torch::autograd::Function<DecayAttention> {
         const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &log_decay = saved[3], &state = saved[4], &start = saved[5];
         at::DeviceGuard guard(q.device());
         Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options()), dstate;
-        if (ctx->saved_data["state"].toBool()) dstate = at::empty(state.sizes(), state.options());
-        if (q.size(1)) {
+        if (ctx->saved_data["state"].toBool() && q.size(0) == 0)
+            dstate = grads[1].defined() ? grads[1].clone(at::MemoryFormat::Contiguous) : at::zeros(state.sizes(), state.options());
+        else if (ctx->saved_data["state"].toBool())
+            dstate = at::empty(state.sizes(), state.options());
+        if (q.size(0) && q.size(1)) {
             Tensor d_out = grads[0].defined() ? rows(grads[0]) : at::zeros(v.sizes(), v.options());
             Tensor d_final = grads[1].defined() ? grads[1].contiguous() : Tensor();
             urgym_ops_seq s = sequence(q, k, v, log_decay, state, start, ctx->saved_data["scale"].toDouble());
@@ -238,8 +244,6 @@ static std::tuple<Tensor, Tensor> decay_attention(const Tensor& q, const Tensor&
     need_start(start, q.sizes().slice(0, 2), q);
     need_gpu(q);
     double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)q.size(3));
-    if (q.size(0) == 0)  // no step: nothing is answered and nothing forgotten
-        return {at::empty(v.sizes(), q.options()), state.defined() ? state.clone(at::MemoryFormat::Contiguous) : at::zeros(shape, q.options().dtype(at::kFloat))};
     Tensor a = rows(q), b = rows(k), c = rows(v), g = log_decay.contiguous();
     if (state.defined()) state = state.contiguous();
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (state.defined() && state.requires_grad()))) {
