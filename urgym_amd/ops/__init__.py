@@ -12,7 +12,8 @@ Tensors are torch tensors on one GPU; every kernel is enqueued on torch's curren
 graph (outputs and workspaces come from torch's allocator, so each captured graph has its own).  When a training step is
 captured, no autograd graph of an earlier eager pass over the same parameters may still be alive: torch ties a parameter's
 gradient accumulation to the stream of the pass that first used it, and joining that stream inside a capture fails.
-Drop the eager outputs first, or capture `torch.autograd.grad`.  Gradients of gradients are not offered.
+Drop the eager outputs first, or capture `torch.autograd.grad`.  Gradients of gradients and forward-mode gradients are not offered,
+nor can a call be traced (torch.jit.trace): each is refused.
 Errors: ValueError / TypeError for arguments, RuntimeError for what the library reports.  There is no CPU fallback.
 """
 import importlib.util

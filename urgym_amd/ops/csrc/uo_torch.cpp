@@ -2,9 +2,11 @@
 // autograd nodes, around the C-ABI of include/urgym_ops.h.  In C++ because a call's own time matters: a rollout step enqueues
 // several of these on a few thousand envs, whose kernels take less time than the same calls from Python do.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <optional>
 
 #include "../../../include/urgym_ops.h"
@@ -34,6 +36,13 @@ static void need_device(const char* name, const Tensor& x, const Tensor& with) {
 
 static void need_gpu(const Tensor& x) {
     TORCH_CHECK_VALUE(x.is_cuda(), "the operators run on the GPU, the tensors are on ", x.device(), "; no CPU fallback exists");
+}
+
+// Refuses what would be lost without a word: the kernels answer no forward-mode tangent, and a trace sees only the outputs' allocation.
+static void need_eager(const char* what, std::initializer_list<const Tensor*> inputs) {
+    for (const Tensor* x : inputs)
+        TORCH_CHECK_VALUE(!x->defined() || !x->_fw_grad(0).defined(), what, ": forward-mode gradients are not offered");
+    TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be traced (torch.jit.trace would record its outputs' allocation only)");
 }
 
 static void* stream_of(const Tensor& x) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index()).stream(); }
@@ -126,6 +135,7 @@ static Tensor layer_norm(const Tensor& x, const Maybe& weight_, const Maybe& bia
     param("bias", bias);
     TORCH_CHECK_TYPE(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(), "weight is ",
                      weight.scalar_type(), ", bias ", bias.scalar_type(), ": one dtype is needed");
+    need_eager("layer_norm", {&x, &weight, &bias});
     need_gpu(x);
     if (at::GradMode::is_enabled() && (x.requires_grad() || (weight.defined() && weight.requires_grad()) || (bias.defined() && bias.requires_grad())))
         return LayerNorm::apply(x, maybe(weight), maybe(bias), eps);
@@ -242,6 +252,7 @@ static std::tuple<Tensor, Tensor> decay_attention(const Tensor& q, const Tensor&
     const int64_t shape[4] = {q.size(1), q.size(2), q.size(3), v.size(3)};
     if (state.defined()) need_state("state", state, shape, q);
     need_start(start, q.sizes().slice(0, 2), q);
+    need_eager("decay_attention", {&q, &k, &v, &log_decay, &state});
     need_gpu(q);
     double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)q.size(3));
     Tensor a = rows(q), b = rows(k), c = rows(v), g = log_decay.contiguous();
@@ -270,6 +281,7 @@ static std::tuple<Tensor, Tensor> decay_attention_step(const Tensor& q, const Te
     TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad() || state.requires_grad() ||
                                                         (out.defined() && out.requires_grad())),
                       "decay_attention_step has no gradient: call it under torch.no_grad(), or decay_attention for training");
+    need_eager("decay_attention_step", {&q, &k, &v, &log_decay, &state, &out});
     need_gpu(q);
     at::DeviceGuard guard(q.device());
     if (out.defined()) out.unsafeGetTensorImpl()->bump_version();  // a graph that has saved it must not use what it becomes
