@@ -62,8 +62,15 @@ class MemoryPolicy(torch.nn.Module):
         self.blocks = torch.nn.ModuleList(_Block(width, heads) for _ in range(layers))
         self.norm = _Norm(width)
         self.head = torch.nn.Linear(width, act_dim)
-        steps = 2.0 * (horizon / 2.0) ** (torch.arange(heads) / max(heads - 1, 1))
+        steps = 2.0 * (horizon / 2.0) ** (torch.arange(heads, dtype=torch.float32) / max(heads - 1, 1))
         self.register_buffer("log_decay", -1.0 / steps)
+
+    def _apply(self, fn, *args, **kw):
+        exact = self.log_decay
+        super()._apply(fn, *args, **kw)
+        if self.log_decay.dtype != exact.dtype:  # the weights' type is converted; decays of another type would be other horizons
+            self.log_decay = exact.to(self.log_decay.device)
+        return self
 
     def initial_state(self, envs):
         """one state per block: nothing remembered"""
@@ -79,7 +86,7 @@ class MemoryPolicy(torch.nn.Module):
     def step(self, obs, state, start=None):
         """obs [envs, obs_dim], state of `initial_state` (updated in place), start [envs] (set where an episode begins):
         actions [envs, act_dim]"""
-        return self._run(obs, lambda i, q, k, v: ops.decay_attention_step(q, k, v, self.log_decay.float(), state[i], start=start,
+        return self._run(obs, lambda i, q, k, v: ops.decay_attention_step(q, k, v, self.log_decay, state[i], start=start,
                                                                           state_out=state[i])[0])
 
     def forward(self, obs, start=None, state=None):
@@ -88,7 +95,7 @@ class MemoryPolicy(torch.nn.Module):
         final = []
 
         def attend(i, q, k, v):
-            o, s = ops.decay_attention(q, k, v, self.log_decay.float(), None if state is None else state[i], start)
+            o, s = ops.decay_attention(q, k, v, self.log_decay, None if state is None else state[i], start)
             final.append(s)
             return o
 
