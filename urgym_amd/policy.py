@@ -49,6 +49,8 @@ class MemoryPolicy(torch.nn.Module):
     """obs_dim -> act_dim with `layers` blocks of decay attention (`heads` heads) of the given width; the heads' horizons (steps
     until the decay has reached 1 / e) run from 2 to `horizon`."""
 
+    has_memory = True  # URGymTorchVecEnv.rollout() steps it
+
     def __init__(self, obs_dim, act_dim, width=128, heads=4, layers=2, horizon=128.0):
         super().__init__()
         if heads < 1 or width % heads:

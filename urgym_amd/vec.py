@@ -156,7 +156,8 @@ class URGymTorchVecEnv:
         return self.obs
 
     def episode_starts(self):
-        """uint8 (n,): 1 where `obs` is the first observation of an episode (after reset(), and after an autoreset)"""
+        """uint8 (n,): 1 where `obs` is the first observation of an episode: after reset(), and after an autoreset.  What is done
+        to `env.sim` directly (set_state, a reset of some envs) it does not see: a policy's state of those envs is cleared by hand."""
         return self.torch.ones_like(self.terminated) if self._fresh else self.terminated | self.truncated
 
     def step(self, actions):
@@ -179,14 +180,16 @@ class URGymTorchVecEnv:
         """Run `policy(obs) -> actions` (a torch module / function on the device) for `steps` batched env steps
         on the env stream; returns per-step reward sums and done counts (tensors on the device).
 
-        A policy with memory -- one that has `initial_state(envs)` and `step(obs, state, start)` -- is stepped with its
+        A policy with memory has `initial_state(envs)`, a list of tensors, and `step(obs, state, start)`, and is stepped with its
         state (updated in place; `state`: what it remembers from the rollout before, None: nothing) and the flags of the
-        envs whose episode begins.  record=True returns a third value, what a learner needs of the rollout as time-major
+        envs whose episode begins.  If it can be called as well, it says so with `has_memory = True`, or `state` is given:
+        otherwise it is called.  record=True returns a third value, what a learner needs of the rollout as time-major
         tensors: "obs" and "action" (float32), "reward", "terminated", "truncated", "start" (uint8, the episode starts
         that `ops.decay_attention` takes), and "state", the memory before the first step (None without memory)."""
         torch = self.torch
-        memory = hasattr(policy, "initial_state") and hasattr(policy, "step")
-        if state is not None and not memory:
+        able = hasattr(policy, "initial_state") and hasattr(policy, "step")
+        memory = able and (state is not None or not callable(policy) or bool(getattr(policy, "has_memory", False)))
+        if state is not None and not able:
             raise TypeError("state is for a policy with memory: one that has initial_state() and step()")
         cur = self._enter()
         with self.stream_context():
