@@ -1,0 +1,66 @@
+"""The policy operators at the sizes that large launches take: 64 columns of the state a wave (heads of 33 to 64, many of them), and the
+widest rows that the layer norm's groups hold -- against the definitions in 64 bits (tests/ops_reference.py)."""
+import pytest
+import torch
+
+from ops_reference import assert_close, decay_bounds, norm_bounds
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+ALL = [torch.float32, torch.bfloat16, torch.float16]
+NAMES = ("o", "final", "dq", "dk", "dv", "dstate")
+
+
+@pytest.fixture(scope="module")
+def ops(built):
+    from urgym_amd import ops
+    return ops
+
+
+@pytest.mark.parametrize("dtype", ALL, ids=str)
+@pytest.mark.parametrize("steps,envs,heads,dk,dv", [(35, 345, 3, 64, 64), (35, 345, 3, 48, 40), (35, 345, 3, 64, 128), (97, 1031, 1, 64, 64),
+                                                    (150, 130, 8, 64, 64), (18, 257, 4, 33, 61), (66, 520, 2, 128, 64), (130, 340, 3, 40, 64)])
+def test_many_heads_of_64(ops, steps, envs, heads, dk, dv, dtype):
+    """(every env is run; the definition is computed for some of them)"""
+    gen = torch.Generator(device=DEV).manual_seed(steps + dk)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV)  # noqa: E731
+    q, k, v, do = (r(steps, envs, heads, d).to(dtype) for d in (dk, dk, dv, dv))
+    state, dfinal = 3 * r(envs, heads, dk, dv), r(envs, heads, dk, dv)
+    decay = torch.log1p(-1.0 / torch.logspace(0.5, 6, heads, base=2.0)).to(DEV) if heads > 1 else torch.tensor([-0.05], device=DEV)
+    start = torch.rand(steps, envs, generator=gen, device=DEV) < 0.04
+    some = torch.tensor([0, 1, envs // 2, envs - 2, envs - 1], device=DEV)
+    for carry, starts in ((state, start), (None, None)):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)] + ([state.detach().requires_grad_()] if carry is not None else [])
+        o, final = ops.decay_attention(*leaves[:3], decay, leaves[3] if carry is not None else None, starts)
+        got = [o, final, *torch.autograd.grad((o, final), leaves, (do, dfinal))]
+        args = [x[:, some] for x in (q, k, v)] + [decay, None if carry is None else carry[some], None if starts is None else starts[:, some]]
+        refs, bounds = decay_bounds(args, dict(do=do[:, some], dfinal=dfinal[some]), dtype)
+        for name, x, ref, b in zip(NAMES, got, refs, bounds):
+            assert torch.isfinite(x.float()).all(), name
+            y = x[some] if name in ("final", "dstate") else x[:, some]
+            assert_close(y, ref, b + (2.0 ** -25 if y.dtype == torch.float16 else 0), (name, carry is None))
+        with torch.no_grad():
+            o2, final2 = ops.decay_attention(q, k, v, decay, carry, starts)
+        assert torch.equal(o2, o) and torch.equal(final2, final)
+
+
+WIDE = [(5, 4095), (5, 8191), (3, 8192), (300, 8184), (3, 12288), (4, 16384), (3, 16392), (3, 32768), (260, 20000), (2, 32776), (600, 4104)]
+
+
+@pytest.mark.parametrize("dtype", ALL, ids=str)
+@pytest.mark.parametrize("rows,width", WIDE)
+def test_layer_norm_of_wide_rows(ops, rows, width, dtype):
+    gen = torch.Generator().manual_seed(width)
+    x = (1.5 * torch.randn(rows, width, generator=gen) + torch.randn(rows, 1, generator=gen)).to(dtype).to(DEV)
+    dy = torch.randn(rows, width, generator=gen).to(dtype).to(DEV)
+    for pdtype in sorted({dtype, torch.float32}, key=str):
+        w = (1 + 0.1 * torch.randn(width, generator=gen)).to(pdtype).to(DEV).requires_grad_()
+        b = (0.1 * torch.randn(width, generator=gen)).to(pdtype).to(DEV).requires_grad_()
+        leaf = x.detach().requires_grad_()
+        y = ops.layer_norm(leaf, w, b)
+        refs, bounds = norm_bounds(x, w, b, 1e-5, dy)
+        for name, a, r, e in zip(("y", "dx", "dw", "db"), (y, *torch.autograd.grad(y, (leaf, w, b), dy)), refs, bounds):
+            assert_close(a, r, e + (2.0 ** -25 if a.dtype == torch.float16 else 0), (name, pdtype))
+        y = ops.layer_norm(x, w, b)
+        (dw,) = torch.autograd.grad(y, (w,), dy)  # without x's gradient
+        assert_close(dw, refs[2], bounds[2] + (2.0 ** -25 if dw.dtype == torch.float16 else 0))
