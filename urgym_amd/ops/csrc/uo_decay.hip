@@ -830,12 +830,13 @@ static int columns_of(int tile, int db, int64_t waves) { return tile == 64 && db
 template <typename T, class L>
 static void launch_tile(const Sweeps& s, hipStream_t st) {
     unsigned grid = (s.items + 7) / 8 * 8;
-    if (s.segs > 1) {
-        k_sweep<T, L, true><<<grid, 64, 0, st>>>(s);
-        unsigned parts = s.items / s.segs * L::VA * L::VB * 2;
-        if (s.segs > 4 * RUNS) k_join<L, 16><<<parts, 256, 0, st>>>(s);
-        else if (s.segs > OWN_JOIN) k_join<L, 4><<<parts, 256, 0, st>>>(s);
-    }
+    if constexpr (L::VB == 2)  // (64 columns are held where the waves fill the chip: in one segment)
+        if (s.segs > 1) {
+            k_sweep<T, L, true><<<grid, 64, 0, st>>>(s);
+            unsigned parts = s.items / s.segs * L::VA * L::VB * 2;
+            if (s.segs > 4 * RUNS) k_join<L, 16><<<parts, 256, 0, st>>>(s);
+            else if (s.segs > OWN_JOIN) k_join<L, 4><<<parts, 256, 0, st>>>(s);
+        }
     k_sweep<T, L, false><<<grid, 64, 0, st>>>(s);
 }
 
