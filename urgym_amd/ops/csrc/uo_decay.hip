@@ -219,10 +219,14 @@ __global__ __launch_bounds__(256) void k_pack(Packs p) {
 }
 
 // 16 bytes at base + each lane's offset to LDS bytes to .. to + 1023, lane by lane.  Written as assembly because the compiler would
-// wait for it before the next read of LDS; the waits are `landed`.  (m0, the address in LDS, has no other use in these kernels.)
+// wait for it before the next read of LDS; the waits are `landed`.  m0 is the address in LDS, and its old value is lost.  (The compiler
+// warns of m0 among the clobbers, that it may not be preserved: that is what is said.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(unsigned to, const void* base, unsigned offset) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Fragments from LDS, as words.  `row`: row t of a tile, the f-th part of it (operand with the dimensions contracted);
