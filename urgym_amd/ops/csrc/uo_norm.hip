@@ -244,7 +244,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_back(int64_t rows, i
     }
 }
 
-// Rows that no group holds (more than 4096 vectors, or 8192 odd elements): a workgroup a row at a time, the row read again for each pass.
+// Rows that no group holds (more than 4096 vectors, backward 2048 in 16 bits, or 8192 odd elements): a workgroup a row at a time, the row read again for each pass.
 template <typename T>
 __global__ __launch_bounds__(1024) void k_norm_wide(int64_t rows, int64_t width, const T* x, int64_t xs, const void* w, const void* b, int wdtype,
                                                     float eps, T* y, float* mean, float* rstd) {
@@ -327,13 +327,15 @@ static int norm_check(const char* what, int dtype, int wdtype, int64_t rows, int
 
 // The group that holds a row of `units` vectors: one vector a thread up to a wave, then more; workgroups of 256 and 1024 threads for
 // wide rows.  Single elements (odd widths) are small work a thread, so a thread takes 4 or 8 of them before the group grows.
-template <bool VECTOR, typename F>
+// No group holds more than MOST.
+template <bool VECTOR, int MOST, typename F>
 static bool norm_group(int64_t units, F&& f) {
 #define TRY(most, G, K) \
-    if (units <= most) { \
-        f.template operator()<G, K>(); \
-        return true; \
-    }
+    if constexpr (most <= MOST) \
+        if (units <= most) { \
+            f.template operator()<G, K>(); \
+            return true; \
+        }
     if constexpr (VECTOR) {
         TRY(8, 8, 1) TRY(16, 16, 1) TRY(32, 32, 1) TRY(64, 64, 1) TRY(128, 64, 2) TRY(256, 256, 1) TRY(512, 256, 2) TRY(768, 256, 3)
         TRY(1024, 256, 4) TRY(2048, 1024, 2) TRY(4096, 1024, 4)
@@ -408,9 +410,9 @@ static int norm_fwd(int64_t rows, int64_t width, const void* x, int64_t xs, cons
     constexpr int V = 16 / sizeof(T);
     bool done;
     if (norm_vectors(width, xs, x, V) && norm_vectors(width, width, y, V) && norm_vectors(width, 0, w, V) && norm_vectors(width, 0, b, V))
-        done = norm_group<true>(width / V, NormForward<T, V>{rows, width, x, xs, w, b, wdtype, eps, y, mean, rstd, st});
+        done = norm_group<true, 4096>(width / V, NormForward<T, V>{rows, width, x, xs, w, b, wdtype, eps, y, mean, rstd, st});
     else
-        done = norm_group<false>(width, NormForward<T, 1>{rows, width, x, xs, w, b, wdtype, eps, y, mean, rstd, st});
+        done = norm_group<false, 8192>(width, NormForward<T, 1>{rows, width, x, xs, w, b, wdtype, eps, y, mean, rstd, st});
     if (!done) k_norm_wide<T><<<norm_blocks(rows, 1, 1024), 1024, 0, st>>>(rows, width, (const T*)x, xs, w, b, wdtype, eps, (T*)y, mean, rstd);
     return uo_launched("urgym_ops_layer_norm");
 }
@@ -422,11 +424,15 @@ static int norm_bwd(int64_t rows, int64_t width, const void* dy, int64_t ds, con
     int64_t parts = norm_parts(rows, width);
     if (!dw && !db) ws = nullptr;
     if (rows && (dx || ws)) {
+        // 4096 vectors of 8 elements and what the gradients need of them are more than 1024 threads' registers: 100 of each thread's
+        // words lay in memory, and such rows are faster read again (bf16, 4096 x 32768: 533 us, 760 held; 4096 x 16392: 273, 536).
+        // Vectors of 4 elements fit but for a few words (float32, 4096 x 16384: 228 us, 347 read again), and so do the forward pass'
+        // (bf16, 4096 x 32768: 140 us, 365).
         bool done;
         if (norm_vectors(width, xs, x, V) && norm_vectors(width, ds, dy, V) && norm_vectors(width, width, dx, V) && norm_vectors(width, 0, w, V))
-            done = norm_group<true>(width / V, NormBackward<T, V>{rows, width, dy, ds, x, xs, w, wdtype, mean, rstd, dx, ws, st});
+            done = norm_group<true, V == 8 ? 2048 : 4096>(width / V, NormBackward<T, V>{rows, width, dy, ds, x, xs, w, wdtype, mean, rstd, dx, ws, st});
         else
-            done = norm_group<false>(width, NormBackward<T, 1>{rows, width, dy, ds, x, xs, w, wdtype, mean, rstd, dx, ws, st});
+            done = norm_group<false, 8192>(width, NormBackward<T, 1>{rows, width, dy, ds, x, xs, w, wdtype, mean, rstd, dx, ws, st});
         if (!done && dx) k_norm_wide_dx<T><<<norm_blocks(rows, 1, 1024), 1024, 0, st>>>(rows, width, (const T*)dy, ds, (const T*)x, xs, w, wdtype, mean, rstd, (T*)dx);
         if (!done && ws)
             k_norm_wide_dw<T><<<dim3((unsigned)parts, (unsigned)((width + 63) / 64)), 64, 0, st>>>(rows, width, (const T*)dy, ds, (const T*)x, xs, mean, rstd, ws);
