@@ -353,14 +353,24 @@ static unsigned norm_blocks(int64_t rows, int per_block, int block) {
     return (unsigned)(n < most ? n : most);
 }
 
-// Workgroups of the backward pass, each of which leaves a part of the column sums (two floats a column, written and read again):
-// about as many as it takes to have 2 MB on the way.  Backward, f16: 512000 x 256 143 us with 768, 151 with 1024, 155 with 512;
-// 10000 x 2048 30 with 512, 39 with 256, 32 with 768; 4097 x 5000 35.5 with 256, 40.5 with 512; single elements, 20000 x 999: 30 with
-// 1024, 40 with 512.
-static int64_t norm_parts(int64_t rows, int64_t width) {
-    int64_t rows_a_time = width <= 512 ? 8 : 1, n = (rows + rows_a_time - 1) / rows_a_time;
-    int64_t most = width <= 512 ? 768 : width % 8 && width <= 2048 ? 1024 : width < 4096 ? 512 : 256;
+// Workgroups of the backward pass, each of which leaves a part of the column sums (two floats a column, written and read again): enough
+// to have 4 to 8 MB on the way, in multiples of the 256 CUs.  `units`: a row's vectors, or 0 where it is taken by single elements.
+// Backward, 48 million elements: float32, rows of 256 with 768 workgroups 115 us, 512 121, 1024 119; of 520, one to a workgroup of
+// half idle threads, with 1024 129, 768 146, 512 186; of 1024 with 768 113, 512 and 1024 120; of 2048 with 512 118, 256 124; of 5000 with 256 119, 512 127;
+// bf16, 1200: 1024 75, 768 82, 512 94; 2048: 768 66, 512 75; 4000: 512 73, 256 82; 8192: 256 80, 512 82.  By single elements, bf16: rows of
+// 999 with 1024 83, 512 112; of 2201 with 512 98, 1024 102; of 5001 with 256 83, 512 88.
+static int64_t norm_parts(int64_t rows, int64_t width, int64_t units) {
+    int64_t rows_a_time = width <= 512 ? 8 : 1, n = (rows + rows_a_time - 1) / rows_a_time, most;
+    if (units) most = units <= 128 ? 768 : units <= 192 ? 1024 : units <= 256 ? 768 : units <= 512 ? 512 : 256;
+    else most = width <= 512 ? 768 : width <= 2048 ? 1024 : width < 4096 ? 512 : 256;
     return n < most ? n : most;
+}
+
+// the most that any type and alignment takes
+static int64_t norm_most_parts(int64_t rows, int64_t width) {
+    int64_t n = norm_parts(rows, width, 0);
+    for (int v = 4; v <= 8; v += 4) n = norm_parts(rows, width, (width + v - 1) / v) > n ? norm_parts(rows, width, (width + v - 1) / v) : n;
+    return n;
 }
 
 template <typename T, int V>
@@ -383,7 +393,7 @@ struct NormForward {
 
 template <typename T, int V>
 struct NormBackward {
-    int64_t rows, width;
+    int64_t rows, width, parts;
     const void* dy;
     int64_t ds;
     const void* x;
@@ -397,7 +407,7 @@ struct NormBackward {
     template <int G, int K>
     void operator()() {
         constexpr int block = G > 256 ? G : 256;
-        k_norm_back<T, G, K, V><<<(unsigned)norm_parts(rows, width), block, 0, st>>>(rows, width, (const T*)dy, ds, (const T*)x, xs, w, wdtype, mean, rstd, (T*)dx, ws);
+        k_norm_back<T, G, K, V><<<(unsigned)parts, block, 0, st>>>(rows, width, (const T*)dy, ds, (const T*)x, xs, w, wdtype, mean, rstd, (T*)dx, ws);
     }
 };
 
@@ -421,7 +431,8 @@ template <typename T>
 static int norm_bwd(int64_t rows, int64_t width, const void* dy, int64_t ds, const void* x, int64_t xs, const void* w, int wdtype,
                     const float* mean, const float* rstd, void* dx, void* dw, void* db, float* ws, hipStream_t st) {
     constexpr int V = 16 / sizeof(T);
-    int64_t parts = norm_parts(rows, width);
+    const bool vectors = norm_vectors(width, xs, x, V) && norm_vectors(width, ds, dy, V) && norm_vectors(width, width, dx, V) && norm_vectors(width, 0, w, V);
+    const int64_t parts = norm_parts(rows, width, vectors ? width / V : 0);
     if (!dw && !db) ws = nullptr;
     if (rows && (dx || ws)) {
         // 4096 vectors of 8 elements and what the gradients need of them are more than 1024 threads' registers: 100 of each thread's
@@ -429,10 +440,10 @@ static int norm_bwd(int64_t rows, int64_t width, const void* dy, int64_t ds, con
         // Vectors of 4 elements fit but for a few words (float32, 4096 x 16384: 228 us, 347 read again), and so do the forward pass'
         // (bf16, 4096 x 32768: 140 us, 365).
         bool done;
-        if (norm_vectors(width, xs, x, V) && norm_vectors(width, ds, dy, V) && norm_vectors(width, width, dx, V) && norm_vectors(width, 0, w, V))
-            done = norm_group<true, V == 8 ? 2048 : 4096>(width / V, NormBackward<T, V>{rows, width, dy, ds, x, xs, w, wdtype, mean, rstd, dx, ws, st});
+        if (vectors)
+            done = norm_group<true, V == 8 ? 2048 : 4096>(width / V, NormBackward<T, V>{rows, width, parts, dy, ds, x, xs, w, wdtype, mean, rstd, dx, ws, st});
         else
-            done = norm_group<false, 8192>(width, NormBackward<T, 1>{rows, width, dy, ds, x, xs, w, wdtype, mean, rstd, dx, ws, st});
+            done = norm_group<false, 8192>(width, NormBackward<T, 1>{rows, width, parts, dy, ds, x, xs, w, wdtype, mean, rstd, dx, ws, st});
         if (!done && dx) k_norm_wide_dx<T><<<norm_blocks(rows, 1, 1024), 1024, 0, st>>>(rows, width, (const T*)dy, ds, (const T*)x, xs, w, wdtype, mean, rstd, (T*)dx);
         if (!done && ws)
             k_norm_wide_dw<T><<<dim3((unsigned)parts, (unsigned)((width + 63) / 64)), 64, 0, st>>>(rows, width, (const T*)dy, ds, (const T*)x, xs, mean, rstd, ws);
@@ -454,7 +465,7 @@ extern "C" int urgym_ops_layer_norm(int dtype, int wdtype, int64_t rows, int64_t
     return NORM_DISPATCH(norm_fwd, rows, width, x, x_stride, weight, bias, wdtype, eps, y, mean, rstd, (hipStream_t)stream);
 }
 
-extern "C" int64_t urgym_ops_layer_norm_workspace(int64_t rows, int64_t width) { return rows < 0 || width < 1 ? 0 : 2 * norm_parts(rows, width) * width; }
+extern "C" int64_t urgym_ops_layer_norm_workspace(int64_t rows, int64_t width) { return rows < 0 || width < 1 ? 0 : 2 * norm_most_parts(rows, width) * width; }
 
 extern "C" int urgym_ops_layer_norm_backward(int dtype, int wdtype, int64_t rows, int64_t width, const void* dy, int64_t dy_stride,
                                              const void* x, int64_t x_stride, const void* weight, const float* mean,
