@@ -92,3 +92,25 @@ def test_layer_norm_workspace_is_enough(ops, width, dtype):
         refs, bounds = norm_bounds(x, w, None, 1e-5, dy)
         for name, a, r, e in zip(("y", "dx", "dw", "db"), (y, dx, dw, db), refs, bounds):
             assert_close(a, r, e + (2.0 ** -25 if a.dtype == torch.float16 else 0), (name, pad))
+
+
+@pytest.mark.parametrize("dtype,steps,envs,dk,dv", [(torch.bfloat16, 31, 300001, 64, 8), (torch.float16, 32, 300001, 8, 128),
+                                                    (torch.float32, 15, 300001, 64, 8), (torch.float32, 16, 300001, 8, 65),
+                                                    (torch.bfloat16, 63, 300001, 65, 9)], ids=str)
+def test_steps_that_lie_far_apart(ops, dtype, steps, envs, dk, dv):
+    """batches whose steps take 150 MB and more: a chunk of them lies over more than 4 GiB"""
+    heads = 4
+    gen = torch.Generator(device=DEV).manual_seed(dk)
+    q, k, v, do = (torch.empty(steps, envs, heads, d, dtype=dtype, device=DEV).normal_(generator=gen) for d in (dk, dk, dv, dv))
+    dfinal = torch.empty(envs, heads, dk, dv, device=DEV).normal_(generator=gen)
+    decay = torch.tensor([-0.5, -0.2, -0.05, -0.01], device=DEV)
+    start = torch.rand(steps, envs, generator=gen, device=DEV) < 0.03
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    o, final = ops.decay_attention(*leaves, decay, None, start)
+    got = [o, final, *torch.autograd.grad((o, final), leaves, (do, dfinal))]
+    some = torch.tensor([0, 1, envs // 2, envs - 1], device=DEV)
+    refs, bounds = decay_bounds([x.detach()[:, some] for x in (q, k, v)] + [decay, None, start[:, some]], dict(do=do[:, some], dfinal=dfinal[some]), dtype)
+    for name, x, ref, b in zip(NAMES, got, refs, bounds):
+        y = x.detach()
+        y = y[some] if name == "final" else y[:, some]
+        assert_close(y, ref, b + (2.0 ** -25 if y.dtype == torch.float16 else 0), name)

@@ -194,11 +194,11 @@ __device__ __forceinline__ u4 padded(const T* p, int col, int width) {
 
 // Tensors whose rows the sweeps cannot load as aligned vectors (odd widths, odd addresses, a chunk over more than 2 GiB) are first
 // copied, rows padded to whole vectors: it costs their bytes three times, but the sweep then runs at its full rate (65 wide heads,
-// bf16, 103 x 1151 x 8: forward 3.2 ms with rows fetched through registers in the sweep).
+// bf16, 103 x 1151 x 8: forward 3.2 ms with rows fetched through registers in the sweep).  A copy in time's order whose chunks lay as
+// far apart has each head's steps together instead.
 struct Packs {
     struct {
-        Rows from;
-        void* to;
+        Rows from, to;
         int width;
     } t[4];
     int count;
@@ -214,8 +214,8 @@ __global__ __launch_bounds__(256) void k_pack(Packs p) {
     if (n >= p.envs) return;
     const int col = i % pieces * N;
     const T* from = (const T*)w.from.p + n * w.from.sn + h * w.from.sh;
-    u4* to = (u4*)w.to + i;
-    for (int64_t t = blockIdx.y; t < p.steps; t += gridDim.y) to[t * p.envs * p.heads * pieces] = padded(from + t * w.from.st, col, w.width);
+    T* to = (T*)w.to.p + n * w.to.sn + h * w.to.sh + col;
+    for (int64_t t = blockIdx.y; t < p.steps; t += gridDim.y) *(u4*)(to + t * w.to.st) = padded(from + t * w.from.st, col, w.width);
 }
 
 // 16 bytes at base + each lane's offset to LDS bytes to .. to + 1023, lane by lane.  Written as assembly because the compiler would
@@ -1031,13 +1031,16 @@ static Sweep backward(const urgym_ops_seq* s, Rows a, Rows b, Rows c, Rows o, in
     return w;
 }
 
+// whether a chunk of rows that lie `st` elements apart is too long for the sweeps' 32-bit offsets
+static bool far(int64_t st, int size) { return (st < 0 ? -st : st) >= ((int64_t)1 << 31) / (32 * size); }
+
 // what the sweeps read of r: itself, or (padded rows, appended to the workspace at `floats`) its copy
 static Rows readable(const urgym_ops_seq* s, Rows r, int d, float* ws, int64_t* floats, Packs* p) {
     int size = s->dtype == URGYM_OPS_F32 ? 4 : 2, n = 16 / size, width = (d + n - 1) / n * n;
-    bool far = (r.st < 0 ? -r.st : r.st) >= ((int64_t)1 << 31) / (32 * size);
-    if (d % n == 0 && (uintptr_t)r.p % 16 == 0 && r.st % n == 0 && r.sn % n == 0 && r.sh % n == 0 && !far) return r;
+    if (d % n == 0 && (uintptr_t)r.p % 16 == 0 && r.st % n == 0 && r.sn % n == 0 && r.sh % n == 0 && !far(r.st, size)) return r;
     Rows to = {ws + *floats, s->envs * s->heads * width, (int64_t)s->heads * width, width};
-    p->t[p->count++] = {r, (void*)to.p, d};
+    if (far(to.st, size)) to = {to.p, width, s->heads * s->steps * width, s->steps * width};
+    p->t[p->count++] = {r, to, d};
     *floats += s->steps * s->envs * s->heads * width * size / 4;
     return to;
 }
