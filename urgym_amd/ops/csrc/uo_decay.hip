@@ -118,9 +118,6 @@ struct Tile {
     static constexpr int DA = DA_, VB = VB_, ES = sizeof(T), FE = 16 / ES, NB = FE / 4, CH = 16 * NB, NF = DA / 4 / FE, VA = DA / 16;
     static constexpr int RA = DA * ES, RC = 16 * VB * ES;  // bytes of a row
     static constexpr int A0 = 0, B0 = CH * RA, C0 = 2 * CH * RA, BUF = 2 * CH * RA + CH * RC;
-    // Rows of 64 bytes (16-bit heads of 32): more than 10 waves a CU slow memory down (512 x 1024 x 4 heads of 32, bf16: 162 us with 16,
-    // 135 with 10 to 13, 138 with 8), so the LDS they are given leaves room for 10.
-    static constexpr int LDS = RA == 64 ? 16384 : BUF;
     // the dimension of row m of C's tile u, and the column (of the wave's) of its column m of tile v: in 16 bits 4 + 4 elements of
     // two tiles are 16 neighbouring bytes, in 32 the tiles' elements alternate
     static __device__ __forceinline__ int dim(int u, int m) { return ES == 2 ? 32 * (u / 2) + 8 * (m / 4) + 4 * (u % 2) + m % 4 : VA * m + u; }
@@ -406,7 +403,7 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
     constexpr int FE = L::FE, NB = L::NB, CH = L::CH, NF = L::NF, VA = L::VA, VB = L::VB, RA = L::RA, RC = L::RC;
     constexpr bool HALF = Kind<T>::HALF;
     constexpr int P = PARTS<T>, TWO = HALF ? 2 : 1;
-    __shared__ __attribute__((aligned(256))) char lds[L::LDS];
+    __shared__ __attribute__((aligned(256))) char lds[L::BUF];
     // workgroups go to the 8 XCDs in turn: each takes a run of items, for neighbours share rows -- the slices, then the sweeps,
     // then the heads of one env -- and their L2
     unsigned item = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
