@@ -28,11 +28,13 @@ extern "C" {
 const char* urgym_ops_last_error(void);
 
 /* y = (x - mean) * rstd * weight + bias over the last axis of x[rows, width] (row stride x_stride; y contiguous).
- * weight / bias: NULL or [width] of dtype wdtype.  mean, rstd: NULL or float32[rows], kept for the backward pass. */
+ * weight / bias: NULL or [width] of dtype wdtype.  mean, rstd: NULL or float32[rows], kept for the backward pass.  width up to
+ * 1 << 20, rows up to 1 << 30. */
 int urgym_ops_layer_norm(int dtype, int wdtype, int64_t rows, int64_t width, const void* x, int64_t x_stride,
                          const void* weight, const void* bias, float eps, void* y, float* mean, float* rstd, void* stream);
 
-/* The float32 elements of workspace that urgym_ops_layer_norm_backward needs for the weight's and bias' gradients. */
+/* The float32 elements of workspace that urgym_ops_layer_norm_backward needs for the weight's and bias' gradients, whatever the types
+ * and alignment. */
 int64_t urgym_ops_layer_norm_workspace(int64_t rows, int64_t width);
 
 /* dx (contiguous, NULL: not wanted), dweight, dbias (both of wdtype, NULL: not wanted) from dy[rows, width] (row stride
@@ -57,8 +59,8 @@ typedef struct {
 } urgym_ops_seq;
 
 /* The float32 elements of workspace (16-byte aligned) that urgym_ops_decay and urgym_ops_decay_backward need for these arguments (0:
- * none, NULL may be passed; <0: error): for copies of tensors whose rows are not whole, aligned 16-byte vectors, and for the
- * states of segments where few heads have many steps. */
+ * none, NULL may be passed; <0: error): for copies of tensors whose rows are not whole, aligned 16-byte vectors or whose steps lie 64 MB
+ * and more apart, and for the states of segments where few heads have many steps. */
 int64_t urgym_ops_decay_workspace(const urgym_ops_seq* s);
 int64_t urgym_ops_decay_backward_workspace(const urgym_ops_seq* s, const void* d_out, const int64_t d_out_stride[3]);
 
@@ -74,7 +76,7 @@ int urgym_ops_decay_backward(const urgym_ops_seq* s, const void* d_out, const in
                              void* stream);
 
 /* One token per env: q, k [envs, heads, dk], v [envs, heads, dv] (strides: env, head), start NULL or uint8 [envs] (stride
- * start_stride); state -> state_out (may be the same buffer), o [envs, heads, dv] contiguous. */
+ * start_stride); state -> state_out (may be the same buffer; apart from all other inputs), o [envs, heads, dv] contiguous. */
 int urgym_ops_decay_step(int dtype, int64_t envs, int heads, int dk, int dv, const void* q, int64_t q_sn, int64_t q_sh,
                          const void* k, int64_t k_sn, int64_t k_sh, const void* v, int64_t v_sn, int64_t v_sh,
                          const float* log_decay, const uint8_t* start, int64_t start_stride, float scale,

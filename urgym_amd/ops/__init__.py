@@ -42,7 +42,7 @@ def _c():
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(variance + eps) * weight + bias over the last axis; statistics and sums in float32.
 
-    x: [..., width] float32, bfloat16 or float16, any strides; weight, bias: [width] of x's dtype or both float32, or None.
+    x: [..., width] float32, bfloat16 or float16, any strides, width up to 1048576; weight, bias: [width] of x's dtype or both float32, or None.
     Returns a contiguous tensor of x's shape and dtype.  Differentiable in x, weight and bias."""
     return (_ext or _c()).layer_norm(x, weight, bias, eps)
 
@@ -59,8 +59,9 @@ def decay_attention(q, k, v, log_decay, state=None, start=None, scale=None):
     a new episode begins -- the step's token does not see what came before it, not even an infinity or NaN.  scale:
     1 / sqrt(dk) if None.
     Returns (o [steps, envs, heads, dv] of q's dtype, the state after the last step).  Products are summed in float32 and
-    the state stays in float32; over more than 32 steps, 16-bit inputs meet the carried state rounded to their own type
-    inside the products for o and the gradients.  What an infinity reaches comes out as infinity or NaN.
+    the state stays in float32.  Products of 16-bit inputs with scores and states take those as two bfloat16 numbers (to 2^-16,
+    whatever their magnitude), three for what the state returned is a sum of; answers are rounded to their type once.
+    What an infinity reaches comes out as infinity or NaN.
     Differentiable in q, k, v and state; backward computes all three of dq, dk, dv."""
     return (_ext or _c()).decay_attention(q, k, v, log_decay, state, start, scale)
 
@@ -68,7 +69,7 @@ def decay_attention(q, k, v, log_decay, state=None, start=None, scale=None):
 def decay_attention_step(q, k, v, log_decay, state, start=None, scale=None, state_out=None):
     """One token per env of `decay_attention`, for a rollout: q, k [envs, heads, dk], v [envs, heads, dv], state float32
     [envs, heads, dk, dv] contiguous, start bool or uint8 [envs].  The new state is written to state_out (`state` itself:
-    in place; None: a new tensor).  Returns (o [envs, heads, dv], the new state).  No gradients: training runs
+    in place; None: a new tensor; another: apart from the other arguments).  Returns (o [envs, heads, dv], the new state).  No gradients: training runs
     `decay_attention` over the recorded steps."""
     return (_ext or _c()).decay_attention_step(q, k, v, log_decay, state, start, scale, state_out)
 

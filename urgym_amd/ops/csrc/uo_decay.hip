@@ -28,11 +28,12 @@
 //   * 16-bit operands that contract the tokens are transposed on their way out of LDS.
 // LDS rows are swizzled in blocks of 16 bytes, so that both kinds of reads spread over the banks.
 //
-// Heads of up to 64 are bound by memory: 500 x 1024 x 4 heads of 64 in bf16 take 260 us forward (1.05 GB: 4.0 TB/s; the same loads and
-// stores without the products 209 to 235) and 520 to 580 backward (dq runs against the time of dk and dv, so its inputs are read
-// again: 7 reads and 3 writes, 2.62 GB, 4.5 to 5.0 TB/s), and fewer waves a CU change nothing until they are 8.  Heads of 128 are bound
-// by the chunk's latency: LDS leaves 8 waves a CU (500 x 4096 heads: 730 us for 2.1 GB; 64 columns a wave are slower yet, 45.6 against
-// 41.8 us at 200 x 512).  So are few heads: a wave alone on its SIMD takes 4 to 5 us a chunk, hence the segments.
+// Heads of up to 64 are bound by memory: 500 x 1024 x 4 heads of 64 in bf16 take 258 to 267 us forward (1.05 GB: 4.0 TB/s; the same loads
+// and stores without the products 209 to 235) and 585 to 631 backward (dq runs against the time of dk and dv, so its inputs are read
+// again: 7 reads and 3 writes, 2.62 GB, 4.2 to 4.5 TB/s; 64 columns leave 2 waves a SIMD, whose conversions of the state and the tokens to
+// parts no longer hide behind them entirely: 516 to 580 with one part less for the state).  Heads of 128 are bound by the chunk's latency:
+// LDS and registers leave 8 waves a CU (500 x 4096 heads, bf16: 755 us for 2.1 GB; float16, whose operands are converted too, 978).  So are
+// few heads: a wave alone on its SIMD takes 4 to 5.5 us a chunk, hence the segments.
 #include "uo_common.h"
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -648,8 +649,8 @@ __global__ __launch_bounds__(64, 2) void k_sweep(Sweeps all) {
         }
 
         // the state: c weighted by its decay to the chunk's end.  In 16 bits the weighted value goes in as two parts (2^-16, enough
-        // for o), and as three where the state itself is an answer, in float32 (forward, 500 x 1024 x 4 heads of 64, bf16: 261 us with
-        // two, 265 with three).  S is touched only where the unit has become small.
+        // for o), and as three where the state itself is an answer, in float32 (bf16, 500 x 1024 x 4 heads of 64: forward 270 us with
+        // two, 271 with three, forward and backward 855 and 880).  S is touched only where the unit has become small.
         float keep = n_tok < CH ? power(lg, n_tok) : whole, unit_new = s_unit * keep;
         const bool off = unit_new < 1.f / 65536 || inside;
         unit_new = off ? 1.f : unit_new;
@@ -824,7 +825,7 @@ __global__ __launch_bounds__(256) void k_join(Sweeps all) {
 constexpr int64_t FILL = 1024;  // waves: one for each SIMD
 
 // Columns of C that a wave holds, by the tile width of a and b and the width of c: as many as its registers take, for they share the
-// scores; 64 with tiles of 64 (500 x 1024 x 4 heads of 64: forward and backward 755 us, 865 with 32), where c has them and the
+// scores; 64 with tiles of 64 (500 x 1024 x 4 heads of 64, bf16: forward and backward 880 us, 1095 with 32), where c has them and the
 // waves fill the chip (with fewer, the time of one wave's chunk counts).
 static int columns_of(int tile, int db, int64_t waves) { return tile == 64 && db > 32 && waves >= FILL ? 64 : 32; }
 
@@ -853,8 +854,8 @@ static int tile(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 // The launch of `count` sweeps, of the widest one's tile.  With fewer waves than fill the chip twice over (one a SIMD is
 // half of that) the axis is cut into segments, at least 32 steps each: their states are computed first, then joined.  That costs a
-// pass, so fewer than 3 segments or 128 steps stay whole (forward, 4 heads of 32, 500 steps, float32: 26 us with 64 steps or more a
-// segment, 21 with 32; 200 heads, 130 steps, bf16: 16.8 us in 2 segments, 13.5 whole).
+// pass, so fewer than 3 segments or 128 steps stay whole (forward, 4 heads of 32, 500 steps, float32: 24 us with 64 steps or more a
+// segment, 20 with 32; 400 heads of 64, 300 steps, bf16: 41 us in 2 segments, 33.5 whole).
 static Sweeps plan(const urgym_ops_seq* q, const Sweep* w, int count) {
     Sweeps s = {};
     s.count = count, s.heads = q->heads, s.steps = q->steps, s.log_decay = q->log_decay;
@@ -1065,8 +1066,10 @@ static Work work(const urgym_ops_seq* s, const Rows* g, float* ws) {
         Rows d = readable(s, *g, s->dv, ws, &w.floats, &w.packs);
         Sweep b[3] = {backward(s, v, d, q, none, s->dv, s->dk, true, nullptr), forward(s, d, v, k, none, s->dv, s->dk, true),
                       backward(s, k, q, d, none, s->dk, s->dv, false, nullptr)};
-        // Tiles of 32 and 64 in 16 bits share the wider one where waves are few and launches count (24 and 40 wide heads, float16, 333 x
-        // 185: 61 -> 49 us, 333 x 370: 91 -> 69, but 333 x 740: 95 -> 106); others never gain (64 and 128, bf16, 333 x 370: 93 -> 125).
+        // Tiles of 32 and 64 in 16 bits share the wider one where waves are few and launches count (24 and 40 wide heads, 333 steps, forward
+        // and backward, bf16 and float16: 185 heads 81 -> 69 and 91 -> 85 us, 370 heads 105 -> 99 and 119 either way, but 740 heads 127 ->
+        // 142 and 151 -> 171); wider ones lose sooner (64 and 128 wide, bf16: 45 heads 80 -> 70, but 185 heads
+        // 117 -> 136, 370 heads 146 -> 188).
         bool few = s->dtype != URGYM_OPS_F32 && s->dk <= 64 && s->dv <= 64 && s->envs * s->heads < FILL / 2;
         if (tile(s->dk) == tile(s->dv) || few) w.sweeps[w.count++] = plan(s, b, 3);
         else w.sweeps[w.count++] = plan(s, b, 2), w.sweeps[w.count++] = plan(s, b + 2, 1);

@@ -24,8 +24,8 @@ extern "C" const char* urgym_ops_last_error(void) { return uo_message; }
 // A row is held by a group of G threads, K vectors of V elements each (V elements = 16 bytes, or 1 where a width, stride or
 // address is odd), so x and dy are read once from memory; the statistics are the mean, then the centred second moment of the
 // values in registers (E[x^2] - mean^2 would cancel).  Groups walk over the rows with the weights kept in registers and the next row
-// already on its way, as it lies in memory (converted on arrival instead, its wait would come at once: 20000 x 999 in f16 40 us backward, 84
-// so).  Both directions are bound by memory: 2 (forward) and 3 (backward) row passes, 512000 x 256 in bf16 in 97 us (5.4
+// already on its way, as it lies in memory (converted on arrival instead, its wait would come at once: 20000 x 999 in f16, 512 workgroups,
+// 40 us backward, 84 so; 30 with norm_parts' workgroups).  Both directions are bound by memory: 2 (forward) and 3 (backward) row passes, 512000 x 256 in bf16 in 97 us (5.4
 // TB/s) and 155 us (5.1 TB/s).
 template <typename T, int V>
 struct Vec {
@@ -354,7 +354,7 @@ static unsigned norm_blocks(int64_t rows, int per_block, int block) {
 }
 
 // Workgroups of the backward pass, each of which leaves a part of the column sums (two floats a column, written and read again): enough
-// to have 4 to 8 MB on the way, in multiples of the 256 CUs.  `units`: a row's vectors, or 0 where it is taken by single elements.
+// to have some MB of rows on the way (4 to 8 for vectors, more for the widest rows), in multiples of the 256 CUs.  `units`: a row's vectors, or 0 where it is taken by single elements.
 // Backward, 48 million elements: float32, rows of 256 with 768 workgroups 115 us, 512 121, 1024 119; of 520, one to a workgroup of
 // half idle threads, with 1024 129, 768 146, 512 186; of 1024 with 768 113, 512 and 1024 120; of 2048 with 512 118, 256 124; of 5000 with 256 119, 512 127;
 // bf16, 1200: 1024 75, 768 82, 512 94; 2048: 768 66, 512 75; 4000: 512 73, 256 82; 8192: 256 80, 512 82.  By single elements, bf16: rows of
